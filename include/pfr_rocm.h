@@ -44,6 +44,7 @@ extern "C" {
 /* Element types; the values are those of pyflame_rt::DType (types.hpp:48-59). */
 typedef enum pfr_dtype {
     PFR_F32 = 0,
+    PFR_F16 = 1, /* the key/value cache and its queries */
     PFR_BF16 = 2,
     PFR_I32 = 5,
     PFR_I8 = 7,
@@ -63,6 +64,7 @@ typedef enum pfr_act {
 typedef struct pfr_ctx pfr_ctx;   /* one device + one stream + scratch */
 typedef struct pfr_csr pfr_csr;   /* device-resident CSR weight */
 typedef struct pfr_sp24 pfr_sp24; /* device-resident 2:4 compressed weight */
+typedef struct pfr_kv pfr_kv;     /* a paged key/value cache over the caller's pools */
 
 /* ---- context ------------------------------------------------------------ */
 
@@ -378,6 +380,89 @@ int pfr_layernorm(pfr_ctx* ctx, const float* x, int64_t outer, int64_t norm,
                   const float* scale, const float* bias, float epsilon, float* y);
 int pfr_layernorm_dev(pfr_ctx* ctx, const float* x, int64_t outer, int64_t norm,
                       const float* scale, const float* bias, float epsilon, float* y);
+
+/* ---- paged key/value cache and attention ----------------------------------- */
+
+/* No counterpart in the reference, which has neither a cache nor attention:
+ * what stands between the q/k/v product and the output product of a decode
+ * layer.  Keys and values of many requests live in two pools of pages (the
+ * caller's memory).  Slot s of a pool is place s % page_size of page s /
+ * page_size; element d of head h of the token there is at
+ *   (s / page_size) * page_stride + h * head_stride
+ *     + (s % page_size) * token_stride + d          (elements)
+ * so that [pages, heads, page_size, dim] and [pages, page_size, heads, dim]
+ * are both served.  A request's block table lists its pages in order.  A prefix
+ * that all requests share is held once, with a table of its own; a request's
+ * own tokens count from 0 after it.
+ *
+ * dtype is PFR_F32, PFR_F16 or PFR_BF16; dim a multiple of 8, at most 256
+ * (PFR_ERR_UNSUPPORTED otherwise); pools and strides multiples of 16 bytes.  The
+ * handle describes the pools and does not own them; it touches no device and
+ * serves every context of the pools' device. */
+int pfr_kv_bind(void* k_pool, void* v_pool, pfr_dtype dtype, int64_t pages, int64_t page_size,
+                int64_t heads, int64_t dim, int64_t page_stride, int64_t head_stride,
+                int64_t token_stride, pfr_kv** out);
+int pfr_kv_info(const pfr_kv* kv, pfr_dtype* dtype, int64_t* pages, int64_t* page_size,
+                int64_t* heads, int64_t* dim);
+int pfr_kv_free(pfr_kv* kv);
+
+/* Block tables and slot maps of a step, on the device.  Request b (of B) holds
+ * cached[b] tokens and gets added[b] more.  The pages it lacks are taken from
+ * free_pages[n_free], request by request, from entry *head on (0 if head is
+ * NULL), and written to its row of table (table_w entries, rows table_ld apart)
+ * behind the ceil(cached / page_size) it has.  Then
+ *   start[b]    tokens added before request b; start[B] all of them
+ *   slots[t]    the slot of added token t (int64); -1 where it has no page, and
+ *               for t from start[B] to max_tokens - 1
+ *   lengths[b]  cached[b] + added[b]
+ *   *head_out   the first entry of free_pages that is still free
+ *   *status     0, or bits: 1 the free list ran out, 2 a request needs more
+ *               than table_w pages, 4 more than max_tokens tokens (start is cut
+ *               to max_tokens), 8 a negative or overflowing count (taken as an
+ *               empty request) or a head outside the list.
+ * Entries of the table other than the new ones keep their values.  lengths,
+ * start and head_out must not overlap cached, added and head: they are the next
+ * step's inputs through other buffers.  All pointers device; one launch. */
+int pfr_kv_tables_dev(pfr_ctx* ctx, const int32_t* cached, const int32_t* added, int64_t B,
+                      int64_t page_size, const int32_t* free_pages, int64_t n_free,
+                      const int32_t* head, int32_t* table, int64_t table_w, int64_t table_ld,
+                      int64_t* slots, int64_t max_tokens, int32_t* start, int32_t* lengths,
+                      int32_t* head_out, int32_t* status);
+
+/* Keys and values of T tokens into their slots.  k and v are [T, heads, dim]
+ * with tokens ldk and ldv elements apart (parts of one fused q/k/v product will
+ * do), float32 (rounded to the cache's type, to nearest even) or of the cache's
+ * type.  Tokens whose slot is negative or past the pool are skipped; slots of one
+ * call must differ.  Device pointers. */
+int pfr_kv_write_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* k, const void* v,
+                     pfr_dtype dtype, int64_t T, int64_t ldk, int64_t ldv, const int64_t* slots);
+
+/* Attention of T tokens.  q and out are [T, heads, dim], tokens ldq and ldo
+ * elements apart, dtype float32 or the cache's type; query head i reads the
+ * cache's head i / (heads / cache heads).  Tokens start[b] .. start[b + 1] - 1
+ * are request b's last ones of lengths[b]: token i of its n sees the prefix
+ * (prefix_len keys through prefix_table) and its own keys 0 .. lengths[b] - n + i:
+ *   out = sum_j w_j V_j / sum_j w_j,  w_j = exp(scale * q . K_j)
+ * with scores, sums and statistics in 32 bits; the weights are rounded to the
+ * cache's type for the product with V where q is 16 bits wide.  The prefix is
+ * read once for all requests, not once for each.
+ * Tokens from start[B] on see the prefix only.  Keys on a page outside the pool
+ * (such as -1) or past the table count as absent; what lies in their place, or in
+ * slots after a request's last token, never reaches a result, and neither does a
+ * key reach the tokens that come before it.  A row without a key, or whose
+ * scores are all -inf, gives zeros.
+ * max_added and max_length bound the tokens and the length of a request as the
+ * caller knows them (0: as many as T and the table allow); they shape the
+ * launch only, and results are right without them.
+ * Partial sums go through the context's grow-only scratch: capture only after
+ * a call of the largest shape.  Device pointers; results do not depend on
+ * timing. */
+int pfr_kv_attention_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* q, pfr_dtype dtype, int64_t T,
+                         int64_t heads, int64_t ldq, float scale, const int32_t* prefix_table,
+                         int64_t prefix_len, const int32_t* table, int64_t table_w,
+                         int64_t table_ld, int64_t B, const int32_t* lengths,
+                         const int32_t* start, int64_t max_added, int64_t max_length, void* out,
+                         int64_t ldo);
 
 /* ---- per-tensor quantize / dequantize ------------------------------------ */
 

@@ -21,7 +21,7 @@ PFR_ERR_HIP = 2
 PFR_ERR_UNSUPPORTED = 3
 PFR_ERR_NO_DEVICE = 4
 
-PFR_F32, PFR_BF16, PFR_I32, PFR_I8, PFR_U8 = 0, 2, 5, 7, 8
+PFR_F32, PFR_F16, PFR_BF16, PFR_I32, PFR_I8, PFR_U8 = 0, 1, 2, 5, 7, 8
 MODE_STRICT, MODE_FAST = 0, 1
 ACT_NONE, ACT_RELU, ACT_GELU = 0, 1, 2
 SP24_OUT_I32, SP24_OUT_F32, SP24_OUT_I8 = 0, 1, 2
@@ -94,6 +94,13 @@ SIGNATURES = {
     "pfr_quantize_linear_dev": (_INT, [_P, _P, _I64, _F, _I32, _INT, _P]),
     "pfr_dequantize_linear": (_INT, [_P, _P, _INT, _I64, _F, _I32, _P]),
     "pfr_dequantize_linear_dev": (_INT, [_P, _P, _INT, _I64, _F, _I32, _P]),
+    "pfr_kv_bind": (_INT, [_P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _PP]),
+    "pfr_kv_info": (_INT, [_P, C.POINTER(_INT), C.POINTER(_I64), C.POINTER(_I64), C.POINTER(_I64), C.POINTER(_I64)]),
+    "pfr_kv_free": (_INT, [_P]),
+    "pfr_kv_tables_dev": (_INT, [_P, _P, _P, _I64, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _P, _P, _P]),
+    "pfr_kv_write_dev": (_INT, [_P, _P, _P, _P, _INT, _I64, _I64, _I64, _P]),
+    "pfr_kv_attention_dev": (_INT, [_P, _P, _P, _INT, _I64, _I64, _I64, _F, _P, _I64, _P, _I64, _I64, _I64, _P, _P,
+                                    _I64, _I64, _P, _I64]),
     "pfr_layernorm": (_INT, [_P, _P, _I64, _I64, _P, _P, _F, _P]),
     "pfr_layernorm_dev": (_INT, [_P, _P, _I64, _I64, _P, _P, _F, _P]),
 }

@@ -1,0 +1,420 @@
+// Paged key/value cache: block tables and slot maps, the write of new tokens,
+// and attention over a prefix that all requests share and their own tokens.
+// None of these has a counterpart in the reference.
+#include <cmath>
+#include <limits>
+
+#include "common.hpp"
+#include "kv.hpp"
+
+#pragma clang fp contract(off)
+
+namespace {
+
+using pfr::FastDiv;
+
+// ---- block tables and slot maps ---------------------------------------------
+
+// Bits of *status.
+constexpr int kNoPages = 1, kNarrowTable = 2, kShortSlots = 4, kBadCount = 8;
+
+constexpr int kTabThreads = 256;  // threads, and requests, per workgroup
+
+struct TablesArgs {
+    const int32_t* cached;
+    const int32_t* added;
+    int32_t B;
+    FastDiv page;
+    const int32_t* free_pages;
+    int32_t n_free;
+    const int32_t* head;
+    int32_t* table;
+    int64_t table_ld;
+    int32_t table_w;
+    int64_t* slots;
+    int32_t max_tokens;
+    int32_t* start;
+    int32_t* lengths;
+    int32_t* head_out;
+    int32_t* status;
+};
+
+// What one request takes: its tokens and pages, and what is wrong with it.
+struct Need {
+    int32_t cached, added, have, pages, bad;
+};
+
+__device__ __forceinline__ Need need_of(const TablesArgs& a, int32_t cached, int32_t added) {
+    Need n;
+    n.bad = (cached < 0 || added < 0 || (int64_t)cached + added > INT32_MAX) ? kBadCount : 0;
+    if (n.bad) {
+        n.cached = 0;
+        n.added = 0;
+    } else {
+        n.cached = cached;
+        n.added = added;
+    }
+    n.have = (int32_t)a.page.div_up((uint32_t)n.cached);
+    const int32_t need = (int32_t)a.page.div_up((uint32_t)n.cached + (uint32_t)n.added);
+    n.pages = need - n.have;
+    if (need > a.table_w) n.bad |= kNarrowTable;
+    return n;
+}
+
+// Sums over the workgroup; every thread gets them.
+__device__ __forceinline__ void block_sum(int64_t& x, int64_t& y, int& bits, int64_t (*sx)[2], int* sb) {
+    for (int o = 32; o; o >>= 1) {
+        x += __shfl_xor(x, o);
+        y += __shfl_xor(y, o);
+        bits |= __shfl_xor(bits, o);
+    }
+    const int w = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+        sx[w][0] = x;
+        sx[w][1] = y;
+        sb[w] = bits;
+    }
+    __syncthreads();
+    x = y = 0;
+    bits = 0;
+    for (int i = 0; i < kTabThreads / 64; ++i) {
+        x += sx[i][0];
+        y += sx[i][1];
+        bits |= sb[i];
+    }
+    __syncthreads();
+}
+
+// The last entry of the ascending s[0 .. n) that is <= v (s[0] <= v).
+__device__ __forceinline__ int last_at_most(const int64_t* s, int n, int64_t v) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s[mid] <= v) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Grid (groups of kTabThreads requests) x (slices of a group's tokens and new
+// pages).  Every workgroup sums what the requests before its group take, scans
+// its own group's, and fills its slice; nothing passes between workgroups, so
+// one launch does it.
+__global__ __launch_bounds__(kTabThreads) void k_kv_tables(TablesArgs a) {
+    __shared__ int64_t tok[kTabThreads + 1], pg[kTabThreads + 1];
+    __shared__ int32_t s_cached[kTabThreads], s_have[kTabThreads];
+    __shared__ int64_t red[kTabThreads / 64][2];
+    __shared__ int redb[kTabThreads / 64];
+    const int tid = threadIdx.x;
+    const int r0 = (int)blockIdx.x * kTabThreads;
+    const bool last_group = blockIdx.x + 1 == gridDim.x;
+
+    int64_t tok0 = 0, pg0 = 0;
+    int bits = 0;
+    for (int r = tid; r < r0; r += kTabThreads) {
+        const Need n = need_of(a, a.cached[r], a.added[r]);
+        tok0 += n.added;
+        pg0 += n.pages;
+        bits |= n.bad;
+    }
+    if (r0 > 0) block_sum(tok0, pg0, bits, red, redb);
+
+    const int r = r0 + tid;
+    const bool mine = r < a.B;
+    Need n = {};
+    if (mine) n = need_of(a, a.cached[r], a.added[r]);
+    // inclusive scans over the group
+    int64_t x = n.added, y = n.pages;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t px = __shfl_up(x, o), py = __shfl_up(y, o);
+        if ((tid & 63) >= o) {
+            x += px;
+            y += py;
+        }
+    }
+    if ((tid & 63) == 63) {
+        red[tid >> 6][0] = x;
+        red[tid >> 6][1] = y;
+    }
+    __syncthreads();
+    for (int w = 0; w < (tid >> 6); ++w) {
+        x += red[w][0];
+        y += red[w][1];
+    }
+    if (tid == 0) tok[0] = pg[0] = 0;
+    tok[tid + 1] = x;
+    pg[tid + 1] = y;
+    s_cached[tid] = n.cached;
+    s_have[tid] = n.have;
+    __syncthreads();
+    const int64_t n_tok = tok[kTabThreads], n_pg = pg[kTabThreads];
+
+    int32_t head = a.head != nullptr ? *a.head : 0;
+    const bool bad_head = head < 0 || head > a.n_free;
+    head = head < 0 ? 0 : (head > a.n_free ? a.n_free : head);
+
+    auto clamp_tok = [&](int64_t t) { return (int32_t)(t < a.max_tokens ? t : a.max_tokens); };
+    if (blockIdx.y == 0) {
+        if (mine) {
+            a.start[r] = clamp_tok(tok0 + tok[tid]);
+            a.lengths[r] = n.cached + n.added;
+        }
+        if (last_group) {
+            int64_t sx = 0, sy = 0;
+            int b = bits | n.bad;
+            block_sum(sx, sy, b, red, redb);
+            if (tid == 0) {
+                const int64_t total = tok0 + n_tok, left = a.n_free - head, taken = pg0 + n_pg;
+                a.start[a.B] = clamp_tok(total);
+                *a.head_out = (int32_t)(head + (taken < left ? taken : left));
+                *a.status = b | (taken > left ? kNoPages : 0) | (total > a.max_tokens ? kShortSlots : 0) |
+                            (bad_head ? kBadCount : 0);
+            }
+        }
+    }
+
+    // the page at place `at` of the sequence of pages taken, -1 past the list
+    auto taken_page = [&](int64_t at) {
+        return at < (int64_t)a.n_free - head ? a.free_pages[head + at] : -1;
+    };
+    const int64_t ny = gridDim.y, sl = blockIdx.y;
+    const int64_t t_lo = n_tok * sl / ny, t_hi = n_tok * (sl + 1) / ny;
+    for (int64_t t = t_lo + tid; t < t_hi && tok0 + t < a.max_tokens; t += kTabThreads) {
+        const int q = last_at_most(tok, kTabThreads, t);
+        const uint32_t p = (uint32_t)s_cached[q] + (uint32_t)(t - tok[q]);
+        const uint32_t j = a.page.div(p), off = p - j * a.page.d;
+        int32_t id = -1;
+        if ((int64_t)j < a.table_w) {
+            if ((int32_t)j < s_have[q]) id = a.table[(int64_t)(r0 + q) * a.table_ld + j];
+            else id = taken_page(pg0 + pg[q] + (int32_t)j - s_have[q]);
+        }
+        a.slots[tok0 + t] = id < 0 ? -1 : (int64_t)id * a.page.d + off;
+    }
+    const int64_t p_lo = n_pg * sl / ny, p_hi = n_pg * (sl + 1) / ny;
+    for (int64_t p = p_lo + tid; p < p_hi; p += kTabThreads) {
+        const int q = last_at_most(pg, kTabThreads, p);
+        const int64_t j = s_have[q] + (p - pg[q]);
+        if (j < a.table_w) a.table[(int64_t)(r0 + q) * a.table_ld + j] = taken_page(pg0 + p);
+    }
+    if (last_group) {
+        const int64_t total = tok0 + n_tok, rest = a.max_tokens - total;
+        if (rest > 0)
+            for (int64_t t = rest * sl / ny + tid; t < rest * (sl + 1) / ny; t += kTabThreads) a.slots[total + t] = -1;
+    }
+}
+
+// ---- the write of new tokens ------------------------------------------------
+
+struct WriteArgs {
+    const void* k;
+    const void* v;
+    int64_t ldk, ldv;  // elements from a token's row to the next
+    const int64_t* slots;
+    int64_t n_slots;   // slots of the pool
+    int64_t nvec;      // 8-element vectors over all tokens
+    FastDiv tok;       // vectors of one token
+    FastDiv head;      // vectors of one head
+    uint32_t page_size;
+    int64_t page_stride, head_stride, token_stride;
+    void* kc;
+    void* vc;
+};
+
+// Eight elements of S rounded to C (to nearest even; the same type: copied).
+template <class S, class C>
+__device__ __forceinline__ void copy8(const S* __restrict__ src, C* __restrict__ dst) {
+    typedef S SV __attribute__((ext_vector_type(8), aligned(sizeof(S))));
+    typedef C CV __attribute__((ext_vector_type(8)));
+    const SV s = *reinterpret_cast<const SV*>(src);
+    *reinterpret_cast<CV*>(dst) = __builtin_convertvector(s, CV);
+}
+
+// One 8-element vector of the keys and of the values per thread.
+template <class S, class C>
+__global__ __launch_bounds__(256) void k_kv_write(WriteArgs a) {
+    const int64_t base = (int64_t)blockIdx.x * 256;
+    const int64_t t0 = base / a.tok.d;  // uniform
+    const uint32_t i = (uint32_t)(base - t0 * a.tok.d) + threadIdx.x;
+    if (base + threadIdx.x >= a.nvec) return;
+    const uint32_t dt = a.tok.div(i), r = i - dt * a.tok.d;
+    const int64_t t = t0 + dt;
+    const int64_t slot = a.slots[t];
+    if (slot < 0 || slot >= a.n_slots) return;
+    const uint32_t h = a.head.div(r), d = (r - h * a.head.d) * 8;
+    const int64_t page = slot / a.page_size, off = slot - page * a.page_size;
+    const int64_t at = page * a.page_stride + (int64_t)h * a.head_stride + off * a.token_stride + d;
+    copy8(static_cast<const S*>(a.k) + t * a.ldk + r * 8, static_cast<C*>(a.kc) + at);
+    copy8(static_cast<const S*>(a.v) + t * a.ldv + r * 8, static_cast<C*>(a.vc) + at);
+}
+
+template <class S>
+void launch_write(hipStream_t s, pfr_dtype cache, unsigned blocks, const WriteArgs& a) {
+    switch (cache) {
+        case PFR_F32: hipLaunchKernelGGL((k_kv_write<S, float>), dim3(blocks), dim3(256), 0, s, a); break;
+        case PFR_F16: hipLaunchKernelGGL((k_kv_write<S, _Float16>), dim3(blocks), dim3(256), 0, s, a); break;
+        default: hipLaunchKernelGGL((k_kv_write<S, __bf16>), dim3(blocks), dim3(256), 0, s, a); break;
+    }
+}
+
+bool is_kv_type(pfr_dtype t) { return t == PFR_F32 || t == PFR_F16 || t == PFR_BF16; }
+int64_t esize(pfr_dtype t) { return t == PFR_F32 ? 4 : 2; }
+
+void tables_dev(pfr_ctx* ctx, const int32_t* cached, const int32_t* added, int64_t B, int64_t page_size,
+                const int32_t* free_pages, int64_t n_free, const int32_t* head, int32_t* table, int64_t table_w,
+                int64_t table_ld, int64_t* slots, int64_t max_tokens, int32_t* start, int32_t* lengths,
+                int32_t* head_out, int32_t* status) {
+    pfr::require(B >= 0 && n_free >= 0 && table_w >= 0 && max_tokens >= 0, "kv tables: negative extent");
+    pfr::require(B <= (1 << 20), "kv tables: at most 2^20 requests");
+    pfr::require(page_size >= 1 && page_size <= (1 << 20), "kv tables: page size must be 1 to 2^20");
+    pfr::require(n_free <= INT32_MAX && table_w <= INT32_MAX && max_tokens <= INT32_MAX, "kv tables: extent above 2^31 - 1");
+    pfr::require(table_ld >= table_w, "kv tables: table row stride below its width");
+    pfr::require(start && head_out && status, "kv tables: null start/head_out/status");
+    pfr::require(B == 0 || (cached && added && lengths), "kv tables: null cached/added/lengths");
+    pfr::require(B == 0 || table_w == 0 || table, "kv tables: null table");
+    pfr::require(max_tokens == 0 || slots, "kv tables: null slots");
+    pfr::require(n_free == 0 || free_pages, "kv tables: null free list");
+    const auto apart = [](const void* x, int64_t xb, const void* y, int64_t yb) {
+        return x == nullptr || y == nullptr || xb == 0 || yb == 0 || pfr::disjoint(x, xb, y, yb);
+    };
+    // every workgroup reads what comes before its own requests
+    pfr::require(apart(cached, 4 * B, lengths, 4 * B) && apart(added, 4 * B, lengths, 4 * B) &&
+                     apart(cached, 4 * B, start, 4 * B + 4) && apart(added, 4 * B, start, 4 * B + 4) &&
+                     apart(head, 4, head_out, 4),
+                 "kv tables: an output overlaps an input");
+    pfr::bind(ctx);
+    TablesArgs a{};
+    a.cached = cached;
+    a.added = added;
+    a.B = (int32_t)B;
+    a.page = FastDiv((uint32_t)page_size);
+    a.free_pages = free_pages;
+    a.n_free = (int32_t)n_free;
+    a.head = head;
+    a.table = table;
+    a.table_ld = table_ld;
+    a.table_w = (int32_t)table_w;
+    a.slots = slots;
+    a.max_tokens = (int32_t)max_tokens;
+    a.start = start;
+    a.lengths = lengths;
+    a.head_out = head_out;
+    a.status = status;
+    const int64_t groups = B == 0 ? 1 : (B + kTabThreads - 1) / kTabThreads;
+    // slices of about 1024 tokens where every group has as many
+    int64_t ny = (max_tokens + groups * 1024 - 1) / (groups * 1024);
+    ny = ny < 1 ? 1 : (ny > 1024 ? 1024 : ny);
+    hipLaunchKernelGGL(k_kv_tables, dim3((unsigned)groups, (unsigned)ny), dim3(kTabThreads), 0, ctx->stream, a);
+    PFR_HIP(hipGetLastError());
+}
+
+void write_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* k, const void* v, pfr_dtype dtype, int64_t T, int64_t ldk,
+               int64_t ldv, const int64_t* slots) {
+    pfr::require(T >= 0, "kv write: negative token count");
+    pfr::require(is_kv_type(dtype), "kv write: keys and values are float32, float16 or bfloat16");
+    if (dtype != PFR_F32 && dtype != kv->dtype)
+        throw pfr::Error(PFR_ERR_UNSUPPORTED, "kv write: 16-bit keys and values go into a cache of their own type");
+    const int64_t row = kv->heads * kv->dim;
+    pfr::require(ldk >= row && ldv >= row, "kv write: token stride below heads * dim");
+    pfr::require(T <= (int64_t(1) << 34) / row, "kv write: too many tokens for one call");
+    pfr::require(T == 0 || (k && v && slots), "kv write: null k/v/slots");
+    pfr::bind(ctx);
+    if (T == 0) return;
+    WriteArgs a{};
+    a.k = k;
+    a.v = v;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.slots = slots;
+    a.n_slots = kv->pages * kv->page_size;
+    a.nvec = T * row / 8;
+    a.tok = FastDiv((uint32_t)(row / 8));
+    a.head = FastDiv((uint32_t)(kv->dim / 8));
+    a.page_size = (uint32_t)kv->page_size;
+    a.page_stride = kv->page_stride;
+    a.head_stride = kv->head_stride;
+    a.token_stride = kv->token_stride;
+    a.kc = kv->k;
+    a.vc = kv->v;
+    const int64_t blocks = (a.nvec + 255) / 256;
+    switch (dtype) {
+        case PFR_F32: launch_write<float>(ctx->stream, kv->dtype, (unsigned)blocks, a); break;
+        case PFR_F16: hipLaunchKernelGGL((k_kv_write<_Float16, _Float16>), dim3((unsigned)blocks), dim3(256), 0, ctx->stream, a); break;
+        default: hipLaunchKernelGGL((k_kv_write<__bf16, __bf16>), dim3((unsigned)blocks), dim3(256), 0, ctx->stream, a); break;
+    }
+    PFR_HIP(hipGetLastError());
+}
+
+}  // namespace
+
+extern "C" {
+
+int pfr_kv_bind(void* k_pool, void* v_pool, pfr_dtype dtype, int64_t pages, int64_t page_size,
+                int64_t heads, int64_t dim, int64_t page_stride, int64_t head_stride, int64_t token_stride,
+                pfr_kv** out) {
+    return pfr::guarded([&] {
+        pfr::require(out != nullptr, "null output handle");
+        *out = nullptr;
+        pfr::require(k_pool && v_pool, "kv cache: null pool");
+        pfr::require(is_kv_type(dtype), "kv cache: pools are float32, float16 or bfloat16");
+        pfr::require(pages >= 1 && heads >= 1 && dim >= 1, "kv cache: empty extent");
+        pfr::require(page_size >= 1 && page_size <= (1 << 20), "kv cache: page size must be 1 to 2^20");
+        pfr::require(pages <= INT32_MAX && heads <= 65536, "kv cache: extent too large");
+        if (dim % 8 != 0 || dim > 256)
+            throw pfr::Error(PFR_ERR_UNSUPPORTED, "kv cache: head dim must be a multiple of 8, at most 256");
+        pfr::require(page_stride >= 0 && head_stride >= 0 && token_stride >= 0, "kv cache: negative stride");
+        pfr::require((heads == 1 || head_stride >= dim) && (page_size == 1 || token_stride >= dim) &&
+                         (pages == 1 || page_stride >= dim),
+                     "kv cache: stride below the head dim");
+        const int64_t vec = 16 / esize(dtype);
+        pfr::require(page_stride % vec == 0 && head_stride % vec == 0 && token_stride % vec == 0 &&
+                         reinterpret_cast<uintptr_t>(k_pool) % 16 == 0 && reinterpret_cast<uintptr_t>(v_pool) % 16 == 0,
+                     "kv cache: pools and strides must be multiples of 16 bytes");
+        auto* kv = new pfr_kv();
+        kv->k = k_pool;
+        kv->v = v_pool;
+        kv->dtype = dtype;
+        kv->pages = pages;
+        kv->page_size = page_size;
+        kv->heads = heads;
+        kv->dim = dim;
+        kv->page_stride = page_stride;
+        kv->head_stride = head_stride;
+        kv->token_stride = token_stride;
+        *out = kv;
+    });
+}
+
+int pfr_kv_info(const pfr_kv* kv, pfr_dtype* dtype, int64_t* pages, int64_t* page_size, int64_t* heads, int64_t* dim) {
+    return pfr::guarded([&] {
+        pfr::require(kv != nullptr, "null kv cache");
+        if (dtype) *dtype = kv->dtype;
+        if (pages) *pages = kv->pages;
+        if (page_size) *page_size = kv->page_size;
+        if (heads) *heads = kv->heads;
+        if (dim) *dim = kv->dim;
+    });
+}
+
+int pfr_kv_free(pfr_kv* kv) {
+    return pfr::guarded([&] { delete kv; });
+}
+
+int pfr_kv_tables_dev(pfr_ctx* ctx, const int32_t* cached, const int32_t* added, int64_t B, int64_t page_size,
+                      const int32_t* free_pages, int64_t n_free, const int32_t* head, int32_t* table, int64_t table_w,
+                      int64_t table_ld, int64_t* slots, int64_t max_tokens, int32_t* start, int32_t* lengths,
+                      int32_t* head_out, int32_t* status) {
+    return pfr::guarded([&] {
+        tables_dev(ctx, cached, added, B, page_size, free_pages, n_free, head, table, table_w, table_ld, slots,
+                   max_tokens, start, lengths, head_out, status);
+    });
+}
+
+int pfr_kv_write_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* k, const void* v, pfr_dtype dtype, int64_t T,
+                     int64_t ldk, int64_t ldv, const int64_t* slots) {
+    return pfr::guarded([&] {
+        pfr::require(kv != nullptr, "null kv cache");
+        write_dev(ctx, kv, k, v, dtype, T, ldk, ldv, slots);
+    });
+}
+
+}  // extern "C"

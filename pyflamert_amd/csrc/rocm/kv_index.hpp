@@ -1,0 +1,86 @@
+// Where a paged cache's keys lie and which of them a token sees: the index
+// arithmetic of its kernels.  Plain C++, so that the host can walk it too.
+#pragma once
+
+#include <cstdint>
+
+#if defined(__HIP__)
+#define PFR_HD __host__ __device__ __forceinline__
+#else
+#define PFR_HD inline
+#endif
+
+namespace pfr {
+
+// x / d for 32-bit x and a d known at launch, by one high product: with s =
+// ceil(log2 d) and m = floor(2^32 (2^s - d) / d) + 1, the quotient is
+// (mulhi(x, m) + x) >> s, the sum taken in 33 bits (Granlund and Montgomery,
+// Division by Invariant Integers using Multiplication, 1994).
+struct FastDiv {
+    uint32_t d = 1, m = 1, s = 0;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t div) : d(div) {
+        while (s < 32 && (uint64_t(1) << s) < d) ++s;
+        m = (uint32_t)((((uint64_t(1) << s) - d) << 32) / d + 1);
+    }
+    PFR_HD uint32_t div(uint32_t x) const {
+        const uint64_t hi = ((uint64_t)x * m) >> 32;
+        return (uint32_t)((hi + x) >> s);
+    }
+    PFR_HD uint32_t div_up(uint32_t x) const {
+        const uint32_t q = div(x);
+        return q + (q * d != x ? 1u : 0u);
+    }
+};
+
+constexpr int kMaxKeys = 1 << 30;  // of one table: key numbers keep room above them in 32 bits
+
+// The geometry of the pools and the tables' reading of it.
+struct PageMap {
+    FastDiv page;       // by the page size
+    uint32_t pages = 0;  // of the pool
+    int64_t page_stride = 0, token_stride = 0;
+};
+
+// The offset of a head's row of key `key` (0 <= key < kMaxKeys), -1 where the table
+// (w entries) ends before it or names no page of the pool.
+PFR_HD int64_t key_offset(const PageMap& m, const int32_t* table, int w, int key) {
+    const uint32_t j = m.page.div((uint32_t)key);
+    if (j >= (uint32_t)w) return -1;
+    const int32_t id = table[j];
+    if ((uint32_t)id >= m.pages) return -1;
+    return (int64_t)id * m.page_stride + (int64_t)((uint32_t)key - j * m.page.d) * m.token_stride;
+}
+
+// Tokens [t0, t1) of request b, within the T there are whatever start holds.
+PFR_HD void request_tokens(const int32_t* start, int b, int T, int* t0, int* t1) {
+    int x = start[b], y = start[b + 1];
+    x = x < 0 ? 0 : (x > T ? T : x);
+    y = y < x ? x : (y > T ? T : y);
+    *t0 = x;
+    *t1 = y;
+}
+
+// Of a request with n new tokens and `length` in all: its first new token sees the
+// keys below first_limit, and each later one a key more.  Lengths are taken
+// within what a table holds.
+PFR_HD int first_limit(int length, int n) {
+    const int len = length < 0 ? 0 : (length > kMaxKeys ? kMaxKeys : length);
+    return len - n + 1;
+}
+
+// The end of the keys that tokens up to the request's new token i see, among the
+// `room` that its table holds.
+PFR_HD int keys_end(int limit0, int i, int64_t room) {
+    const int64_t end = (int64_t)limit0 + i;
+    return (int)(end < 0 ? 0 : (end > room ? room : end));
+}
+
+// Keys [*lo, *hi) of split s of n: `chunk` a split, the last one takes what is left.
+PFR_HD void split_span(int s, int n, int chunk, int end, int* lo, int* hi) {
+    const int64_t at = (int64_t)s * chunk;
+    *lo = at < end ? (int)at : end;
+    *hi = s + 1 == n || end - *lo < chunk ? end : *lo + chunk;
+}
+
+}  // namespace pfr

@@ -205,6 +205,31 @@ class Context:
     def layernorm_dev(self, x_ptr, outer, norm, scale_ptr, bias_ptr, epsilon, y_ptr):
         check(self._lib.pfr_layernorm_dev(self.handle, x_ptr, outer, norm, scale_ptr, bias_ptr, float(epsilon), y_ptr))
 
+    # -- paged key/value cache ---------------------------------------------
+    def kv_bind(self, k_ptr, v_ptr, dtype, pages, page_size, heads, dim, page_stride=None, head_stride=None,
+                token_stride=None):
+        """Paged key/value cache over the caller's pools (pfr_kv_bind), dtype
+        "f32", "f16" or "bf16".  Strides in elements; left out: contiguous
+        [pages, heads, page_size, dim]."""
+        if token_stride is None:
+            token_stride = dim
+        if head_stride is None:
+            head_stride = page_size * token_stride
+        if page_stride is None:
+            page_stride = heads * head_stride
+        h = C.c_void_p()
+        check(self._lib.pfr_kv_bind(k_ptr, v_ptr, _kv_type(dtype), pages, page_size, heads, dim, page_stride,
+                                    head_stride, token_stride, C.byref(h)))
+        return KvCache(self, h)
+
+    def kv_tables_dev(self, cached_ptr, added_ptr, B, page_size, free_ptr, n_free, head_ptr, table_ptr, table_w,
+                      slots_ptr, max_tokens, start_ptr, lengths_ptr, head_out_ptr, status_ptr, table_ld=None):
+        """Block tables and slot maps of a step (pfr_kv_tables_dev), device
+        pointers; slots are int64, everything else int32."""
+        check(self._lib.pfr_kv_tables_dev(self.handle, cached_ptr, added_ptr, B, page_size, free_ptr, n_free, head_ptr,
+                                          table_ptr, table_w, table_w if table_ld is None else table_ld, slots_ptr,
+                                          max_tokens, start_ptr, lengths_ptr, head_out_ptr, status_ptr))
+
     # -- per-tensor quantize / dequantize ----------------------------------
     def quantize_linear(self, x, scale, zero_point=0, out="i8"):
         """quantize_tensor with per-tensor parameters: int8 (out="i8") or
@@ -406,3 +431,56 @@ class Sp24Weight:
     def gemm_bf16_dev(self, X_ptr, N, Y_ptr, ldx=None, ldy=None):
         check(self.ctx._lib.pfr_sp24_gemm_bf16_dev(self.ctx.handle, self.handle, X_ptr, N, ldx or N, Y_ptr,
                                                    ldy or N))
+
+
+_KV_TYPES = {"f32": _lib.PFR_F32, "f16": _lib.PFR_F16, "bf16": PFR_BF16}
+
+
+def _kv_type(name):
+    try:
+        return _KV_TYPES[name]
+    except KeyError:
+        raise TypeError('keys, values and queries are "f32", "f16" or "bf16"') from None
+
+
+class KvCache:
+    """Paged key/value cache over the caller's pools (pfr_kv).  It keeps their
+    addresses, not the tensors: hold those as long as the cache."""
+
+    def __init__(self, ctx, handle):
+        self.ctx = ctx
+        self.handle = handle
+        dt = C.c_int()
+        n = [C.c_int64() for _ in range(4)]
+        check(ctx._lib.pfr_kv_info(handle, C.byref(dt), *(C.byref(x) for x in n)))
+        self.dtype = dt.value
+        self.pages, self.page_size, self.heads, self.dim = (x.value for x in n)
+
+    def free(self):
+        if self.handle:
+            check(self.ctx._lib.pfr_kv_free(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+    def write_dev(self, k_ptr, v_ptr, T, slots_ptr, dtype, ldk=None, ldv=None):
+        """Keys and values of T tokens into their slots (pfr_kv_write_dev)."""
+        row = self.heads * self.dim
+        check(self.ctx._lib.pfr_kv_write_dev(self.ctx.handle, self.handle, k_ptr, v_ptr, _kv_type(dtype), T,
+                                             row if ldk is None else ldk, row if ldv is None else ldv, slots_ptr))
+
+    def attention_dev(self, q_ptr, T, heads, out_ptr, dtype, scale=None, prefix_table_ptr=None, prefix_len=0,
+                      table_ptr=None, table_w=0, B=0, lengths_ptr=None, start_ptr=None, max_added=0, max_length=0,
+                      ldq=None, ldo=None, table_ld=None):
+        """Attention of T tokens over the shared prefix and their requests' own
+        keys (pfr_kv_attention_dev); scale None: 1 / sqrt(dim)."""
+        row = heads * self.dim
+        check(self.ctx._lib.pfr_kv_attention_dev(
+            self.ctx.handle, self.handle, q_ptr, _kv_type(dtype), T, heads, row if ldq is None else ldq,
+            self.dim ** -0.5 if scale is None else scale, prefix_table_ptr, prefix_len, table_ptr, table_w,
+            table_w if table_ld is None else table_ld, B, lengths_ptr, start_ptr, max_added, max_length, out_ptr,
+            row if ldo is None else ldo))
