@@ -1,0 +1,874 @@
+// Attention over a paged key/value cache: what its kernels share, and the
+// kernels themselves; kv_attn_*.hip instantiate them for a pair of types each.
+#pragma once
+
+#include <type_traits>
+
+#include "common.hpp"
+#include "kv.hpp"
+
+#pragma clang fp contract(off)
+
+namespace pfr {
+namespace attn {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 4;       // waves of a workgroup
+constexpr int kBlock = 32;      // keys of a wave's block, narrow form
+constexpr int kWideRows = 128;  // rows of a workgroup, wide form: 32 a wave
+constexpr int kWideKeys = 64;   // keys of its tile
+
+struct Args {
+    const void* q;
+    int64_t ldq;
+    void* out;
+    int64_t ldo;
+    const void* k;
+    const void* v;
+    int64_t head_stride;
+    PageMap map;
+    FastDiv group;  // by the query heads of a key head
+    int32_t D, G, Hkv, Hq;
+    int32_t T;
+    float scale;  // |scale of the scores| log2 e, 1 for a scale of 0
+    float sign;   // its sign, applied to q
+    const int32_t* prefix_table;
+    int32_t prefix_len;
+    const int32_t* table;
+    int64_t table_ld;
+    int32_t table_w;
+    const int32_t* lengths;
+    const int32_t* start;
+    int32_t B;
+    // Apart: p_items = Hkv * p_tiles * p_splits workgroups for the prefix, p_chunk
+    // keys a split, its tiles over the rows of all tokens; then Hkv * B *
+    // o_tiles * o_splits for the requests' own keys, o_chunk a split.
+    // Together (whole): a request's tiles see the prefix and then its own
+    // keys; splits are of that whole range.
+    int32_t whole, p_items, p_tiles, p_splits, p_chunk, o_tiles, o_splits, o_chunk;
+    float* part_o;    // [p_splits + o_splits][T * Hq][D], null: rows are whole after one workgroup
+    float2* part_ml;  // [p_splits + o_splits][T * Hq]: largest score (log2 units), sum of weights
+};
+
+// The kernels of a call: narrow (kNarrow1, 2: 16 or 32 rows, waves share the
+// keys), wide (128 rows, waves share the tile), or the prefix wide and own keys narrow.
+enum Kind { kNarrow1, kNarrow2, kMixed1, kMixed2, kWide };
+
+template <class QT, class KT>
+void launch(hipStream_t s, const Args& a, Kind kind, unsigned blocks);
+
+// Keys [lo, hi) of a table of w entries.
+struct Seg {
+    const int32_t* table;
+    int w, lo, hi;
+};
+
+template <class T>
+struct Mfma16;
+template <>
+struct Mfma16<__bf16> {
+    typedef __bf16 V8 __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f4 dot(V8 a, V8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f16v dot32(V8 a, V8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Mfma16<_Float16> {
+    typedef _Float16 V8 __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f4 dot(V8 a, V8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f16v dot32(V8 a, V8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+
+template <int BYTES>
+struct Raw;
+template <>
+struct Raw<8> {
+    typedef u2 T;
+};
+template <>
+struct Raw<16> {
+    typedef u4 T;
+};
+
+template <class T>
+constexpr uint32_t exp_bits() {
+    return sizeof(T) == 4 ? 0x7f800000u : (std::is_same<T, _Float16>::value ? 0x7c00u : 0x7f80u);
+}
+
+// q times the sign of the scale (1, -1 or 0), exact.
+template <class V>
+__device__ __forceinline__ V signed_q(V q, float sign) {
+    if (sign != 1.0f) {
+#pragma unroll
+        for (int e = 0; e < (int)(sizeof(V) / sizeof(q[0])); ++e) q[e] = (decltype(q[0] + q[0]))((float)q[e] * sign);
+    }
+    return q;
+}
+
+// The operands of one block of kBlock keys and RT tiles of 16 query rows, and
+// the running output, in registers.  Lane = 16 g + n.
+//
+// Scores are S^T = K Q^T, 16 keys x 16 rows a tile: the matrix unit leaves row
+// n's scores of keys 4 g + i of the tile in the lane's registers i.  That is
+// where the second product, O^T = V^T P^T, wants its right operand if its
+// sum runs over the keys in the order (g; tile 0's 4 g .. 4 g + 3, tile 1's),
+// so P goes from one product into the other without leaving its lane, and a
+// row's statistics, its P and its O^T column share the lane's n.
+template <class QT, class KT, int DP, int RT, bool FULL>
+struct Tiles {
+    static constexpr bool kHalf = sizeof(QT) == 2;         // 16-bit products; else float32 ones
+    static constexpr int VE = 16 / (int)sizeof(KT);         // elements of a 16-byte load
+    static constexpr int KS = DP / (4 * VE);                // key loads per lane and tile
+    static constexpr int VV = VE < DP / 16 ? VE : DP / 16;  // contiguous values of a lane per load
+    static constexpr int CC = DP / 16 / VV;                 // value loads per lane and key
+    static constexpr int NT = DP / 16;                      // 16-wide column tiles of O: tile c * VV + e
+    typedef typename Raw<VV * (int)sizeof(KT)>::T VRaw;
+    typedef QT QV __attribute__((ext_vector_type(VE)));
+    typedef QT QVu __attribute__((ext_vector_type(VE), aligned(sizeof(QT))));
+    typedef KT KV __attribute__((ext_vector_type(VE)));
+
+    QV q[RT][KS];
+    KV k[2][KS];
+    VRaw v[8][CC];
+    f4 o[RT][NT];
+
+    // element e of load s of a lane is d = (4 s + g) VE + e, for rows of Q and of K alike
+    __device__ __forceinline__ void load_q(int rt, const QT* row, bool valid, int g, int D, float sign) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = (4 * s + g) * VE;
+            q[rt][s] = QV(0);
+            if (valid && (FULL || d < D)) q[rt][s] = signed_q(QV(*reinterpret_cast<const QVu*>(row + d)), sign);
+        }
+    }
+    __device__ __forceinline__ void load_k(int t, const KT* row, int g, int D) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = (4 * s + g) * VE;
+            if (FULL || d < D) k[t][s] = *reinterpret_cast<const KV*>(row + d);
+            else k[t][s] = KV(0);
+        }
+    }
+    // value register j is key 4 g + j of tile 0 (j < 4) or 4 g + j - 4 of tile
+    // 1, columns (16 c + n) VV ..
+    __device__ __forceinline__ void load_v(int j, const KT* row, int n, int D) {
+#pragma unroll
+        for (int c = 0; c < CC; ++c) {
+            const int d = (16 * c + n) * VV;
+            if (FULL || d < D) v[j][c] = *reinterpret_cast<const VRaw*>(row + d);
+            else v[j][c] = VRaw(0);
+        }
+    }
+    __device__ __forceinline__ void zero_v(int j) {
+#pragma unroll
+        for (int c = 0; c < CC; ++c) v[j][c] = VRaw(0);
+    }
+    // whether value register j holds an infinity or a NaN
+    __device__ __forceinline__ bool nonfinite_v(int j) const {
+        constexpr uint32_t E = exp_bits<KT>();
+        bool bad = false;
+#pragma unroll
+        for (int c = 0; c < CC; ++c)
+#pragma unroll
+            for (int w = 0; w < (int)sizeof(VRaw) / 4; ++w) {
+                const uint32_t x = v[j][c][w];
+                bad |= (x & E) == E;
+                if constexpr (sizeof(KT) == 2) bad |= ((x >> 16) & E) == E;
+            }
+        return bad;
+    }
+    __device__ __forceinline__ f4 scores(int rt, int t) const {
+        f4 acc = f4(0.0f);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if constexpr (kHalf) {
+                acc = Mfma16<KT>::dot(k[t][s], q[rt][s], acc);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VE; ++e)
+                    acc = __builtin_amdgcn_mfma_f32_16x16x4f32((float)k[t][s][e], q[rt][s][e], acc, 0, 0, 0);
+            }
+        }
+        return acc;
+    }
+    // o += V^T p for the lane's eight keys, p in the order of v's registers.
+    // With 16-bit products p is rounded to the cache's type (its error, half a
+    // step a weight and averaged over the keys, is the size of the output's
+    // own rounding); the sum of the weights keeps 32 bits.
+    __device__ __forceinline__ void add(int rt, const float (&p)[8]) {
+        if constexpr (kHalf) {
+            typename Mfma16<KT>::V8 pv;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) pv[j] = (KT)p[j];
+#pragma unroll
+            for (int c = 0; c < CC; ++c)
+#pragma unroll
+                for (int e = 0; e < VV; ++e) {
+                    // the lane's column e of its eight keys, two keys a register
+                    u4 col;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        col[x] = __builtin_amdgcn_perm(v[2 * x + 1][c][e / 2], v[2 * x][c][e / 2],
+                                                       (e & 1) ? 0x07060302u : 0x05040100u);
+                    o[rt][c * VV + e] = Mfma16<KT>::dot(__builtin_bit_cast(typename Mfma16<KT>::V8, col), pv, o[rt][c * VV + e]);
+                }
+        } else {
+            typedef KT VK __attribute__((ext_vector_type(VV)));
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int c = 0; c < CC; ++c) {
+                    const VK x = __builtin_bit_cast(VK, v[j][c]);
+#pragma unroll
+                    for (int e = 0; e < VV; ++e)
+                        o[rt][c * VV + e] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x[e], p[j], o[rt][c * VV + e], 0, 0, 0);
+                }
+        }
+    }
+};
+
+// The largest over the four lanes that hold a row.
+__device__ __forceinline__ float row_max(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float row_sum(float x) {
+    x = x + __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// Whether four 16-bit values hold an infinity or a NaN.
+template <class T>
+__device__ __forceinline__ bool nonfinite(unsigned a, unsigned b) {
+    constexpr uint32_t E = exp_bits<T>();
+    return (a & E) == E || ((a >> 16) & E) == E || (b & E) == E || ((b >> 16) & E) == E;
+}
+
+// A 64-bit value that all lanes hold, in scalar registers.
+__device__ __forceinline__ unsigned long long uniform(unsigned long long x) {
+    return (unsigned)__builtin_amdgcn_readfirstlane((int)x) |
+           (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+}
+
+// The value of the lane 32 away.
+__device__ __forceinline__ float half_swap(float x) {
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// Four 16-bit elements a lane of a tile in the LDS, transposed among 16 lanes:
+// lane i gets element i % 4 of what lanes i / 4, i / 4 + 4, .. + 12 address.
+__device__ __forceinline__ s4 read_tr(const char* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
+}
+
+// One workgroup's rows against keys [lo, hi) of one table.  Rows r0 .. of the
+// n_rows that start at token t0: row r is query head r % G of token t0 + r / G.
+// lim0 and per_token: row r sees keys below lim0 + per_token * (r / G).
+// Writes the rows' part `part`.
+template <class QT, class KT, int DP, int RT, bool FULL>
+__device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0, int r0, int n_rows,
+                                       const Seg& seg, int lim0, int per_token, int part) {
+    const int32_t* __restrict__ table = seg.table;
+    const int table_w = seg.w, lo = seg.lo, hi = seg.hi;
+    typedef Tiles<QT, KT, DP, RT, FULL> TT;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    TT x;
+    float m[RT], l[RT];
+    int lim[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r = r0 + rt * 16 + n;
+        const bool valid = r < n_rows;
+        const int dt = (int)a.group.div((uint32_t)(valid ? r : 0));
+        const int hq = h * a.G + (valid ? r : 0) - dt * a.G;
+        x.load_q(rt, static_cast<const QT*>(a.q) + (int64_t)(t0 + dt) * a.ldq + (int64_t)hq * a.D, valid, g, a.D, a.sign);
+        lim[rt] = valid ? lim0 + per_token * dt : 0;
+        m[rt] = -INFINITY;
+        l[rt] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < TT::NT; ++i) x.o[rt][i] = f4(0.0f);
+    }
+    // all rows see the keys below this
+    const int min_lim = lim0 + per_token * (int)a.group.div((uint32_t)r0);
+    const KT* kp = static_cast<const KT*>(a.k) + (int64_t)h * a.head_stride;
+    const KT* vp = static_cast<const KT*>(a.v) + (int64_t)h * a.head_stride;
+
+    for (int k0 = lo + w * kBlock; k0 < hi; k0 += kWaves * kBlock) {
+        // lane i (and i + 32) finds key i
+        const int key = k0 + (lane & 31);
+        int64_t off = key < hi ? key_offset(a.map, table, table_w, key) : -1;
+        const uint32_t okm = (uint32_t)__ballot(off >= 0);
+        off = off < 0 ? 0 : off;  // the pool's first row is there to be read
+        if (okm == 0) continue;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) x.load_k(t, kp + __shfl((long long)off, 16 * t + n), g, a.D);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x.load_v(u, vp + __shfl((long long)off, (u < 4 ? 0 : 16) + 4 * g + (u & 3)), n, a.D);
+
+        const bool partly = k0 + kBlock > min_lim;
+        uint32_t poison = 0;
+        if (okm != ~0u) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (!((okm >> ((u < 4 ? 0 : 16) + 4 * g + (u & 3))) & 1)) x.zero_v(u);
+        }
+        if (partly) {
+            // A key that only some rows see must not reach the others, and 0
+            // times an infinity or a NaN would: such values are added row by row.
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const uint64_t b = __ballot(x.nonfinite_v(u));
+#pragma unroll
+                for (int gg = 0; gg < 4; ++gg)
+                    if ((b >> (16 * gg)) & 0xffff) poison |= 1u << ((u < 4 ? 0 : 16) + 4 * gg + (u & 3));
+            }
+            if (min_lim > k0) poison &= ~0u << (min_lim - k0);
+            if (poison) {
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if ((poison >> ((u < 4 ? 0 : 16) + 4 * g + (u & 3))) & 1) x.zero_v(u);
+            }
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            float s[8];
+            const f4 s0 = x.scores(rt, 0), s1 = x.scores(rt, 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[i] = s0[i];
+                s[4 + i] = s1[i];
+            }
+            if (partly || okm != ~0u) {
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int kk = (u < 4 ? 0 : 16) + 4 * g + (u & 3);
+                    if (!((okm >> kk) & 1) || k0 + kk >= lim[rt]) s[u] = -INFINITY;
+                }
+            }
+            float mx = s[0];
+#pragma unroll
+            for (int u = 1; u < 8; ++u) mx = fmaxf(mx, s[u]);
+            const float mn = fmaxf(m[rt], row_max(mx) * a.scale), ms = finite_max(mn);
+            const float alpha = __builtin_amdgcn_exp2f(m[rt] - ms);
+            m[rt] = mn;
+            float p[8], sum = 0.0f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                p[u] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u], a.scale, -ms));
+                sum = sum + p[u];
+            }
+            l[rt] = l[rt] * alpha + sum;
+#pragma unroll
+            for (int i = 0; i < TT::NT; ++i) x.o[rt][i] *= alpha;
+            x.add(rt, p);
+            for (uint32_t rest = poison; rest; rest &= rest - 1) {
+                const int kk = __builtin_ctz(rest), u0 = (kk >> 4) * 4 + (kk & 3), g0 = (kk >> 2) & 3;
+                float mine = 0.0f;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) mine = u == u0 ? p[u] : mine;
+                const float pk = __shfl(mine, 16 * g0 + n);
+                const KT* row = vp + __shfl((long long)off, kk);
+                if (((okm >> kk) & 1) && k0 + kk < lim[rt]) {
+#pragma unroll
+                    for (int c = 0; c < TT::CC; ++c)
+#pragma unroll
+                        for (int e = 0; e < TT::VV; ++e)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int d = (16 * c + 4 * g + i) * TT::VV + e;
+                                if (FULL || d < a.D) x.o[rt][c * TT::VV + e][i] += pk * (float)row[d];
+                                if (i == 3) __builtin_amdgcn_sched_barrier(0);  // not all of them in registers at once
+                            }
+                }
+            }
+        }
+    }
+
+    // the waves' sums, joined
+    float* sm = lds;                       // [kWaves][16 RT] maxima
+    float* sl = lds + kWaves * 16 * RT;    // [kWaves][16 RT] sums
+    float* so = lds + 2 * kWaves * 16 * RT;  // [kWaves][16][64 VV's columns + 4]
+    constexpr int kCols = 16 * TT::VV, kPitch = kCols + 4;
+    __syncthreads();
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        l[rt] = row_sum(l[rt]);
+        if (g == 0) {
+            sm[w * 16 * RT + rt * 16 + n] = m[rt];
+            sl[w * 16 * RT + rt * 16 + n] = l[rt];
+        }
+    }
+    __syncthreads();
+    const int64_t rows_all = (int64_t)a.T * a.Hq;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        if (r0 + rt * 16 >= n_rows) break;
+        float M = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) M = fmaxf(M, sm[i * 16 * RT + rt * 16 + n]);
+        const float f = __builtin_amdgcn_exp2f(m[rt] - finite_max(M));
+        if (w == 0 && g == 0 && r0 + rt * 16 + n < n_rows) {
+            float L = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i)
+                L = L + sl[i * 16 * RT + rt * 16 + n] * __builtin_amdgcn_exp2f(sm[i * 16 * RT + rt * 16 + n] - finite_max(M));
+            const int r = r0 + rt * 16 + n, dt = (int)a.group.div((uint32_t)r);
+            const int64_t R = (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G);
+            a.part_ml[(int64_t)part * rows_all + R] = make_float2(M, L);
+        }
+#pragma unroll
+        for (int c = 0; c < TT::CC; ++c) {
+            float* mine = so + w * 16 * kPitch + n * kPitch;
+#pragma unroll
+            for (int e = 0; e < TT::VV; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mine[(4 * g + i) * TT::VV + e] = x.o[rt][c * TT::VV + e][i] * f;
+            __syncthreads();
+            for (int z = threadIdx.x; z < 16 * kCols; z += kWaves * 64) {
+                const int rr = z / kCols, cc = z % kCols, r = r0 + rt * 16 + rr, d = c * kCols + cc;
+                if (r < n_rows && d < a.D) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < kWaves; ++i) sum = sum + so[i * 16 * kPitch + rr * kPitch + cc];
+                    const int dt = (int)a.group.div((uint32_t)r);
+                    const int64_t R = (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G);
+                    a.part_o[((int64_t)part * rows_all + R) * a.D + d] = sum;
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+template <int RT>
+constexpr int lds_floats(int cols) {
+    return 2 * kWaves * 16 * RT + kWaves * 16 * (cols + 4);
+}
+
+
+
+// ---- wide form: 32 rows a wave, tiles of keys through the LDS ---------------------
+
+template <int DP>
+struct WideLds {
+    static constexpr int kRow = DP > 64 ? 256 : 128;  // bytes of a key's row
+    alignas(16) char k[2][kWideKeys * kRow];
+    alignas(16) char v[2][kWideKeys * kRow];
+    int64_t off[3][kWideKeys];  // the keys' offsets, -1: absent
+    unsigned long long ok[3];     // which are there
+    uint8_t poison[3][kWideKeys];  // which hold a value that is no number
+};
+
+template <class T, int DP, bool FULL>
+__device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int t0, int r0, int n_rows, const Seg& pre,
+                                     const Seg& own, int lim0, int part) {
+    typedef typename Mfma16<T>::V8 V8;
+    typedef V8 V8u __attribute__((aligned(2)));
+    typedef T V4 __attribute__((ext_vector_type(4)));
+    constexpr int kRow = WideLds<DP>::kRow;
+    constexpr int CPR = DP / 8;   // 16-byte chunks of a key's row
+    constexpr int LPT = DP / 32;  // chunks of K, and of V, a thread moves per tile
+    constexpr int QS = DP / 16, DB = DP / 32, KG = QS / 2;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = lane & 31, hh = lane >> 5;
+    const int np = (pre.hi - pre.lo + kWideKeys - 1) / kWideKeys;
+    const int nt = np + (own.hi - own.lo + kWideKeys - 1) / kWideKeys;
+
+    // the lane's row
+    const int r = r0 + 32 * w + n;
+    const bool valid = r < n_rows;
+    const int dt = (int)a.group.div((uint32_t)(valid ? r : n_rows - 1));
+    const int hq = h * a.G + (valid ? r : n_rows - 1) - dt * a.G;
+    const int lim = lim0 + dt;
+    const bool wave_valid = r0 + 32 * w < n_rows;
+    // in the own keys: all rows of the workgroup (of the wave) see those below
+    const int min_lim = lim0 + (int)a.group.div((uint32_t)r0);
+    const int wave_min = __builtin_amdgcn_readfirstlane(lim), wave_max = __builtin_amdgcn_readlane(lim, 31);
+
+    V8 q[QS];
+    {
+        const T* row = static_cast<const T*>(a.q) + (int64_t)(t0 + dt) * a.ldq + (int64_t)hq * a.D;
+#pragma unroll
+        for (int s = 0; s < QS; ++s) {
+            const int d = 16 * s + 8 * hh;
+            q[s] = V8(0);
+            if (FULL || d < a.D) q[s] = signed_q(V8(*reinterpret_cast<const V8u*>(row + d)), a.sign);
+        }
+    }
+    f16v o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i) o[i] = f16v(0.0f);
+    float m = -INFINITY, l = 0.0f;
+
+    const T* kp = static_cast<const T*>(a.k) + (int64_t)h * a.head_stride;
+    const T* vp = static_cast<const T*>(a.v) + (int64_t)h * a.head_stride;
+    u4 kr[LPT], vr[LPT];
+
+    const auto tile_key = [&](int i) { return i < np ? pre.lo + kWideKeys * i : own.lo + kWideKeys * (i - np); };
+    // one wave finds the keys of tile i
+    const auto lookup = [&](int i, int slot) {
+        const bool p = i < np;
+        const int key = tile_key(i) + lane;
+        const int64_t off = key < (p ? pre.hi : own.hi) ? key_offset(a.map, p ? pre.table : own.table, p ? pre.w : own.w, key) : -1;
+        lds.off[slot][lane] = off;
+        const unsigned long long ok = __ballot(off >= 0);
+        if (lane == 0) lds.ok[slot] = ok;
+        lds.poison[slot][lane] = 0;
+    };
+    const auto load = [&](int slot) {
+#pragma unroll
+        for (int j = 0; j < LPT; ++j) {
+            const int id = tid + 256 * j, key = id / CPR, c = id % CPR;
+            const int64_t off = lds.off[slot][key];
+            // an absent key: the pool's first row is there to be read, and so is a row's first chunk
+            const int64_t at = (off < 0 ? 0 : off) + (FULL || c * 8 < a.D ? c * 8 : 0);
+            kr[j] = *reinterpret_cast<const u4*>(kp + at);
+            vr[j] = *reinterpret_cast<const u4*>(vp + at);
+        }
+    };
+    // Rows of a tile are kRow bytes apart; chunk c of row x is kept at c ^ (x &
+    // 15) for K, whose products read a chunk of 16 rows at a time, and c ^ 4 (x
+    // & 3) for V, whose transposed reads take 4 rows x 4 chunks: neither
+    // meets a bank twice (64-element rows: two to 256 bytes, the same by pairs).
+    const auto store = [&](int i, int slot, int buf) {
+        const unsigned long long ok = uniform(lds.ok[slot]);
+        const bool partly = i >= np && tile_key(i) + kWideKeys > min_lim;
+        if (ok != ~0ull || partly) {
+#pragma unroll
+            for (int j = 0; j < LPT; ++j) {
+                const int key = (tid + 256 * j) / CPR;
+                if (!((ok >> key) & 1)) vr[j] = u4(0);
+                if (partly) {
+                    // four values with one that is no number: kept from the rows that do not see them, see below
+                    const bool x = nonfinite<T>(vr[j][0], vr[j][1]), y = nonfinite<T>(vr[j][2], vr[j][3]);
+                    if (x) vr[j][0] = vr[j][1] = 0;
+                    if (y) vr[j][2] = vr[j][3] = 0;
+                    if (x || y) lds.poison[slot][key] = 1;
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < LPT; ++j) {
+            const int id = tid + 256 * j, key = id / CPR, c = id % CPR;
+            const int fk = kRow == 256 ? key & 15 : (key >> 1) & 7, fv = kRow == 256 ? (key & 3) << 2 : ((key >> 1) & 1) << 2;
+            if (!FULL && c * 8 >= a.D) kr[j] = vr[j] = u4(0);
+            *reinterpret_cast<u4*>(lds.k[buf] + key * kRow + ((c ^ fk) << 4)) = kr[j];
+            *reinterpret_cast<u4*>(lds.v[buf] + key * kRow + ((c ^ fv) << 4)) = vr[j];
+        }
+    };
+
+    if (nt > 0) {
+        if (w < 2 && w < nt) lookup(w, w);
+        __syncthreads();
+        load(0);
+        store(0, 0, 0);
+        __syncthreads();
+    }
+    const int kat = n * kRow + (((kRow == 256 ? n & 15 : (n >> 1) & 7) ^ hh) << 4);
+    // transposed read: lane 4 e + x of 16 holds row e's columns 4 x .., and lane
+    // i gets column i of the four rows
+    const int vrow = 4 * hh + ((lane & 15) >> 2);
+    const int vsw = kRow == 256 ? vrow & 3 : (vrow >> 1) & 1;
+    const int vat = vrow * kRow + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) << 4) + (lane & 1) * 8;
+
+    int slot = 0;
+    for (int i = 0; i < nt; ++i) {
+        const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot1 == 2 ? 0 : slot1 + 1, buf = i & 1;
+        if (i + 1 < nt) load(slot1);
+        if (i + 2 < nt && w == (i & 3)) lookup(i + 2, slot2);
+        const int k0 = tile_key(i);
+        const bool mine = i >= np;
+        if (wave_valid && (!mine || k0 < wave_max)) {
+            const char* kb = lds.k[buf];
+            const char* vb = lds.v[buf];
+            f16v s[2];
+            // Four groups of fragments of K, then of V, each read while the one before is multiplied.
+            V8 kf[2][KG];
+            const auto read_k = [&](int g) {
+#pragma unroll
+                for (int j = 0; j < KG; ++j)
+                    kf[g & 1][j] = *reinterpret_cast<const V8*>(kb + (g >> 1) * 32 * kRow + (kat ^ ((j + (g & 1) * KG) << 5)));
+            };
+            read_k(0);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (g < 3) read_k(g + 1);
+#pragma unroll
+                for (int j = 0; j < KG; ++j)
+                    s[g >> 1] = Mfma16<T>::dot32(kf[g & 1][j], q[j + (g & 1) * KG], (g & 1) == 0 && j == 0 ? f16v(0.0f) : s[g >> 1]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const unsigned long long ok = uniform(lds.ok[slot]);
+            if (ok != ~0ull || (mine && k0 + kWideKeys > wave_min)) {
+                const int see = mine ? lim - k0 : kWideKeys;
+                unsigned long long there = ok & (see >= kWideKeys ? ~0ull : (see <= 0 ? 0ull : (1ull << see) - 1));
+                there >>= 4 * hh;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x)
+                        s[b][x] = (unsigned)(there >> 32 * b) & (1u << (8 * (x >> 2) + (x & 3))) ? s[b][x] : -INFINITY;
+            }
+            float mx = s[0][0];
+#pragma unroll
+            for (int x = 1; x < 16; ++x) mx = fmaxf(mx, s[0][x]);
+#pragma unroll
+            for (int x = 0; x < 16; ++x) mx = fmaxf(mx, s[1][x]);
+            mx = fmaxf(mx, half_swap(mx));
+            const float mn = fmaxf(m, mx * a.scale), ms = finite_max(mn);
+            if (__any(mn > m)) {
+                const float alpha = __builtin_amdgcn_exp2f(m - ms);
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[d] *= alpha;
+                m = mn;
+            }
+            V8 p[2][2];
+            float sum = 0.0f;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][x], a.scale, -ms));
+                    sum = sum + e;
+                    p[b][x >> 3][x & 7] = (T)e;
+                }
+            l = l + sum;
+            V8 vf[2][DB];
+            const auto read_v = [&](int g) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    const char* at = vb + 16 * g * kRow + vat + ((d ^ vsw) << 6);
+                    const s4 lo = read_tr(at), hi = read_tr(at + 8 * kRow);
+                    vf[g & 1][d] = __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+            };
+            read_v(0);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (g < 3) read_v(g + 1);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[d] = Mfma16<T>::dot32(vf[g & 1][d], p[g >> 1][g & 1], o[d]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            unsigned long long poison = mine && k0 + kWideKeys > min_lim ? __ballot(lds.poison[slot][lane] != 0) : 0;
+            // A key that only some rows see must not reach the others, and 0 times
+            // an infinity or a NaN would: such values are added row by row.
+            for (; poison; poison &= poison - 1) {
+                const int kk = __builtin_ctzll(poison), at = ((kk >> 3) & 3) * 4 + (kk & 3);
+                float pk = 0.0f;
+#pragma unroll
+                for (int x = 0; x < 16; ++x) pk = x == at ? (float)(kk < 32 ? p[0][x >> 3][x & 7] : p[1][x >> 3][x & 7]) : pk;
+                pk = __shfl(pk, (kk & 4) * 8 + n);
+                const T* row = vp + lds.off[slot][kk];
+                if (k0 + kk < lim) {
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int c = 32 * d + 8 * j + 4 * hh;
+                            if (FULL || c < a.D) {
+                                const V4 x = *reinterpret_cast<const V4*>(row + c);
+                                const u2 y = __builtin_bit_cast(u2, x);
+                                if (nonfinite<T>(y[0], y[1])) {
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) o[d][4 * j + e] += pk * (float)x[e];
+                                }
+                            }
+                            __builtin_amdgcn_sched_barrier(0);  // not all of them in registers at once
+                        }
+                }
+            }
+        }
+        if (i + 1 < nt) store(i + 1, slot1, buf ^ 1);
+        __syncthreads();
+        slot = slot1;
+    }
+
+    if (!valid) return;
+    l = l + half_swap(l);
+    const int64_t R = (int64_t)(t0 + dt) * a.Hq + hq;
+    if (part < 0) {
+        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+        typedef T T4u __attribute__((ext_vector_type(4), aligned(2)));
+        T* row = static_cast<T*>(a.out) + (int64_t)(t0 + dt) * a.ldo + (int64_t)hq * a.D;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = 32 * d + 8 * j + 4 * hh;
+                if (FULL || c < a.D) {
+                    T4u x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = (T)(o[d][4 * j + e] * f);
+                    *reinterpret_cast<T4u*>(row + c) = x;
+                }
+            }
+        return;
+    }
+    const int64_t at = (int64_t)part * a.T * a.Hq + R;
+    if (hh == 0) a.part_ml[at] = make_float2(m, l);
+    float* row = a.part_o + at * a.D;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = 32 * d + 8 * j + 4 * hh;
+            if (FULL || c < a.D) {
+                f4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = o[d][4 * j + e];
+                *reinterpret_cast<f4*>(row + c) = x;
+            }
+        }
+}
+
+// ---- the kernels --------------------------------------------------------------------
+
+// What a workgroup does.
+struct Item {
+    int h, b, tile, split;  // b < 0: the prefix, for all tokens
+};
+__device__ __forceinline__ Item item_of(const Args& a) {
+    int i = (int)blockIdx.x;
+    Item x;
+    if (i < a.p_items) {
+        x.h = i % a.Hkv;
+        i /= a.Hkv;
+        x.b = -1;
+        x.tile = i % a.p_tiles;
+        x.split = i / a.p_tiles;
+        return x;
+    }
+    i -= a.p_items;
+    const int nb = a.B + (a.whole ? 2 : 0);
+    x.h = i % a.Hkv;
+    i /= a.Hkv;
+    x.tile = i % a.o_tiles;
+    i /= a.o_tiles;
+    x.b = i % nb;
+    x.split = i / nb;
+    return x;
+}
+
+// No keys for rows [r0, r1) of a part: the join skips what has no weight.
+__device__ __forceinline__ void no_keys(const Args& a, int h, int t0, int r0, int r1, int part) {
+    for (int r = r0 + (int)threadIdx.x; r < r1; r += kWaves * 64) {
+        const int dt = (int)a.group.div((uint32_t)r);
+        a.part_ml[(int64_t)part * a.T * a.Hq + (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G)] = make_float2(-INFINITY, 0.0f);
+    }
+}
+
+// DN, FULL, RT: the narrow form's; DW, WF: the wide form's (0: there is none);
+// OWN: whether a request's own keys take the wide form too.
+template <class QT, class KT, int DN, bool FULL, int RT, int DW, bool WF, bool OWN>
+__device__ __forceinline__ void attention(const Args& a, char* lds) {
+    const Item x = item_of(a);
+    const bool prefix = x.b < 0;
+    int t0 = 0, t1 = a.T, lim0 = a.prefix_len, P = a.prefix_len, part = x.split, tiles_apart = a.p_tiles;
+    int64_t room = 0;
+    const int32_t* table = nullptr;
+    if (!prefix) {
+        if (a.whole) tokens_of(a.start, a.B, x.b, a.T, &t0, &t1);
+        else request_tokens(a.start, x.b, a.T, &t0, &t1);
+        const bool listed = x.b < a.B;  // else tokens of no request
+        lim0 = 0;
+        if (listed) {
+            lim0 = first_limit(a.lengths[x.b], t1 - t0);
+            room = (int64_t)a.table_w * a.map.page.d;
+            table = a.table + (int64_t)x.b * a.table_ld;
+        }
+        if (!a.whole) P = 0;
+        part = a.part_o == nullptr ? -1 : a.p_splits + x.split;
+        tiles_apart = a.o_tiles;
+    }
+    const int n_rows = (t1 - t0) * a.G;
+    const int splits = prefix ? a.p_splits : a.o_splits, chunk = prefix ? a.p_chunk : a.o_chunk;
+    const bool use_wide = OWN || (DW > 0 && prefix);
+    const int rows = use_wide ? kWideRows : 16 * RT;
+    for (int tile = x.tile; tile * (int64_t)rows < n_rows; tile += tiles_apart) {
+        const int r0 = tile * rows, r1 = r0 + rows < n_rows ? r0 + rows : n_rows;
+        const int end = prefix ? 0 : keys_end(lim0, (int)a.group.div((uint32_t)(r1 - 1)), room);
+        int lo, hi;  // of the prefix and the own keys behind it
+        split_span(x.split, splits, chunk, P + end, &lo, &hi);
+        if (part >= 0 && lo == hi) {
+            no_keys(a, x.h, t0, r0, r1, part);
+            continue;
+        }
+        const Seg pre{a.prefix_table, INT32_MAX, lo < P ? lo : P, hi < P ? hi : P};
+        const Seg own{table, a.table_w, lo > P ? lo - P : 0, hi > P ? hi - P : 0};
+        if constexpr (OWN) {
+            wide<QT, DW, WF>(a, *reinterpret_cast<WideLds<DW>*>(lds), x.h, t0, r0, n_rows, pre, own, lim0, part);
+        } else if constexpr (DW > 0) {
+            if (prefix) wide<QT, DW, WF>(a, *reinterpret_cast<WideLds<DW>*>(lds), x.h, t0, r0, n_rows, pre, Seg{nullptr, 0, 0, 0}, 0, part);
+            else narrow<QT, KT, DN, RT, FULL>(a, reinterpret_cast<float*>(lds), x.h, t0, r0, n_rows, own, lim0, 1, part);
+            __syncthreads();
+        } else {
+            narrow<QT, KT, DN, RT, FULL>(a, reinterpret_cast<float*>(lds), x.h, t0, r0, n_rows, prefix ? pre : own, lim0, prefix ? 0 : 1, part);
+            __syncthreads();
+        }
+    }
+}
+
+template <class QT, class KT, int DN, bool FULL, int RT>
+constexpr int narrow_lds() {
+    return 4 * lds_floats<RT>(16 * Tiles<QT, KT, DN, RT, FULL>::VV);
+}
+
+template <class QT, class KT, int D, bool FULL, int RT>
+__global__ __launch_bounds__(kWaves * 64, RT == 1 && D < 256 ? 2 : 1) void k_attn_narrow(Args a) {
+    __shared__ __attribute__((aligned(16))) char lds[narrow_lds<QT, KT, D, FULL, RT>()];
+    attention<QT, KT, D, FULL, RT, 0, false, false>(a, lds);
+}
+
+template <class T, int DN, bool FULL, int RT, int DW, bool WF>
+__global__ __launch_bounds__(kWaves * 64, 2) void k_attn_mixed(Args a) {
+    constexpr int x = narrow_lds<T, T, DN, FULL, RT>(), y = (int)sizeof(WideLds<DW>);
+    __shared__ __attribute__((aligned(16))) char lds[x > y ? x : y];
+    attention<T, T, DN, FULL, RT, DW, WF, false>(a, lds);
+}
+
+template <class T, int DW, bool WF>
+__global__ __launch_bounds__(kWaves * 64, 2) void k_attn_wide(Args a) {
+    __shared__ __attribute__((aligned(16))) char lds[sizeof(WideLds<DW>)];
+    attention<T, T, 64, false, 1, DW, WF, true>(a, lds);
+}
+
+template <class QT, class KT, int DN, bool FULL, int DW, bool WF>
+void launch_kind(hipStream_t s, const Args& a, Kind kind, unsigned blocks) {
+    const dim3 grid(blocks), wg(kWaves * 64);
+    if constexpr (DW > 0) {
+        if (kind == kMixed1) { hipLaunchKernelGGL((k_attn_mixed<QT, DN, FULL, 1, DW, WF>), grid, wg, 0, s, a); return; }
+        if (kind == kMixed2) { hipLaunchKernelGGL((k_attn_mixed<QT, DN, FULL, 2, DW, WF>), grid, wg, 0, s, a); return; }
+        if (kind == kWide) { hipLaunchKernelGGL((k_attn_wide<QT, DW, WF>), grid, wg, 0, s, a); return; }
+    }
+    if constexpr (DN < 256) {
+        if (kind == kNarrow2) { hipLaunchKernelGGL((k_attn_narrow<QT, KT, DN, FULL, 2>), grid, wg, 0, s, a); return; }
+    }
+    hipLaunchKernelGGL((k_attn_narrow<QT, KT, DN, FULL, 1>), grid, wg, 0, s, a);
+}
+
+template <class QT, class KT>
+void launch(hipStream_t s, const Args& a, Kind kind, unsigned blocks) {
+    constexpr bool half = sizeof(QT) == 2;
+    if (a.D == 128) launch_kind<QT, KT, 128, true, half ? 128 : 0, true>(s, a, kind, blocks);
+    else if (a.D == 64) launch_kind<QT, KT, 64, true, half ? 64 : 0, true>(s, a, kind, blocks);
+    else if (a.D < 64) launch_kind<QT, KT, 64, false, half ? 64 : 0, false>(s, a, kind, blocks);
+    else if (a.D == 96) launch_kind<QT, KT, 128, false, half ? 96 : 0, true>(s, a, kind, blocks);
+    else if (a.D < 96) launch_kind<QT, KT, 128, false, half ? 96 : 0, false>(s, a, kind, blocks);
+    else if (a.D < 128) launch_kind<QT, KT, 128, false, half ? 128 : 0, false>(s, a, kind, blocks);
+    else launch_kind<QT, KT, 256, false, 0, false>(s, a, kind, blocks);
+}
+
+}  // namespace attn
+}  // namespace pfr

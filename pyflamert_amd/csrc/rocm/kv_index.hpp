@@ -61,6 +61,15 @@ PFR_HD void request_tokens(const int32_t* start, int b, int T, int* t0, int* t1)
     *t1 = y;
 }
 
+// The same, and for b = B the tokens from start[B] on, for b = B + 1 those before
+// start[0]: all T of them where start ascends.
+PFR_HD void tokens_of(const int32_t* start, int B, int b, int T, int* t0, int* t1) {
+    if (b < B) return request_tokens(start, b, T, t0, t1);
+    const int x = b == B ? start[B] : start[0], at = x < 0 ? 0 : (x > T ? T : x);
+    *t0 = b == B ? at : 0;
+    *t1 = b == B ? T : at;
+}
+
 // Of a request with n new tokens and `length` in all: its first new token sees the
 // keys below first_limit, and each later one a key more.  Lengths are taken
 // within what a table holds.
