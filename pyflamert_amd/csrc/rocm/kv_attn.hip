@@ -42,15 +42,23 @@ __global__ __launch_bounds__(256) void k_kv_attn_join(Args a) {
     const int step = pair ? 2 : 1, half = pair ? lane >> 5 : 0, d = 4 * (pair ? lane & 31 : lane);
     const float* src = a.part_o + R * a.D + d;
     f4 acc = f4(0.0f);
-#pragma unroll 4
-    for (int p0 = 0; p0 < parts; p0 += step) {
-        const int p = p0 + half;
-        const float fp = __shfl(f, p);
-        if (((live >> p) & 1) && d < a.D) {
-            const f4 x = *reinterpret_cast<const f4*>(src + p * rows * a.D);
+    constexpr int kAtOnce = 4;
+    for (int p0 = 0; p0 < parts; p0 += step * kAtOnce) {
+        f4 x[kAtOnce];
+        float fp[kAtOnce];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = acc[e] + fp * x[e];
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int p = p0 + i * step + half;
+            fp[i] = __shfl(f, p);
+            const bool there = p < 64 && ((live >> p) & 1) && d < a.D;
+            x[i] = f4(0.0f);
+            if (there) x[i] = *reinterpret_cast<const f4*>(src + p * rows * a.D);
+            else fp[i] = 0.0f;
         }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = acc[e] + fp[i] * x[i][e];
     }
     if (pair) {
 #pragma unroll
@@ -69,6 +77,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Splits of `keys` keys, each of `chunk` keys (a multiple of `round`), for
 // about `want` of them, and at most kMaxParts.
 constexpr int kMaxParts = 24;
+#define SOLO_CHUNK 256
 void split_keys(int64_t want, int64_t round, int64_t keys, int32_t* splits, int32_t* chunk) {
     int64_t s = ceil_div(keys, round);
     s = want < s ? want : s;
@@ -78,37 +87,66 @@ void split_keys(int64_t want, int64_t round, int64_t keys, int32_t* splits, int3
     *chunk = (int32_t)c;
 }
 
-// Which kernels, and how the work is cut into workgroups.
-Kind plan(int num_cu, bool half, int64_t max_added, int64_t max_length, int64_t room, Args& a) {
-    const int64_t rows = (int64_t)a.T * a.G, own_rows = max_added * a.G;  // of a key head
-    const bool can_wide = half && a.D <= 128, can_two = a.D <= 128;
-    const bool own_wide = can_wide && a.B > 0 && own_rows > 32;
-    const int64_t slots = 2 * num_cu;  // workgroups at a time
+// The kernels of a call and their workgroups; one launch where both parts take the same kernel.
+struct Plan {
+    Kind prefix = pfr::attn::kNarrow1, own = pfr::attn::kNarrow1;
+    int64_t prefix_blocks = 0, own_blocks = 0;
+};
 
-    a.whole = own_wide && rows >= 2 * kWideRows * a.B && a.prefix_len + room < INT32_MAX - 4096;
+// Which kernels, and how the work is cut into workgroups.
+Plan plan(int num_cu, bool half, int64_t max_added, int64_t max_length, int64_t room, Args& a) {
+    using namespace pfr::attn;
+    Plan p;
+    const int64_t rows = (int64_t)a.T * a.G, own_rows = max_added * a.G;  // of a key head
+    const auto kind = [&](int64_t n) { return half && a.D <= 128 && n > 32 ? kWide : (a.D <= 128 && n > 16 ? kNarrow2 : kNarrow1); };
+    const auto tile = [](Kind k) { return k == kWide ? kWideRows : (k == kNarrow2 ? 32 : 16); };
+    const int64_t slots = 2 * num_cu;  // workgroups at a time
+    const int64_t round = kWaves * kBlock, wide_round = 4 * kWideKeys;
+
+    p.own = kind(own_rows);
+    a.whole = a.B > 0 && p.own == kWide && rows >= 2 * kWideRows * a.B && a.prefix_len + room < INT32_MAX - 4096;
     if (a.whole) {
         a.o_tiles = (int32_t)ceil_div(own_rows, kWideRows);
         const int64_t tiles = a.Hkv * (rows / kWideRows + a.B);
-        split_keys(tiles >= slots ? 1 : ceil_div(slots, tiles), 4 * kWideKeys, a.prefix_len + max_length, &a.o_splits, &a.o_chunk);
+        split_keys(tiles >= slots ? 1 : ceil_div(slots, tiles), wide_round, a.prefix_len + max_length, &a.o_splits, &a.o_chunk);
         if (a.o_splits == 0) a.o_splits = 1;
     } else {
-        const bool p_wide = can_wide && (own_wide || rows > 32);
-        const int rt = can_two && ((!p_wide && rows > 16) || (!own_wide && a.B > 0 && own_rows > 16)) ? 2 : 1;
-        a.p_tiles = (int32_t)ceil_div(rows, p_wide ? kWideRows : 16 * rt);
-        const int64_t round = kWaves * kBlock;
-        split_keys(ceil_div(slots, (int64_t)a.Hkv * a.p_tiles), p_wide ? 4 * kWideKeys : round, a.prefix_len, &a.p_splits, &a.p_chunk);
-        a.p_items = a.Hkv * a.p_tiles * a.p_splits;
+        p.prefix = kind(rows);
         if (a.B > 0) {
-            a.o_tiles = (int32_t)ceil_div(own_rows, own_wide ? kWideRows : 16 * rt);
-            split_keys(ceil_div(2 * slots, (int64_t)a.Hkv * a.B * a.o_tiles), own_wide ? 4 * kWideKeys : round, max_length, &a.o_splits, &a.o_chunk);
+            // one kernel for both where it costs no more than half of its rows
+            if (p.prefix != kWide && p.own != kWide) p.prefix = p.own = p.prefix > p.own ? p.prefix : p.own;
+            a.o_tiles = (int32_t)ceil_div(own_rows, tile(p.own));
+            const int64_t own = (int64_t)a.Hkv * a.B * a.o_tiles;
+            if (p.own != kWide && own * ceil_div(max_length, SOLO_CHUNK) >= 2 * kWaves * slots) {
+                a.solo = 1;
+                split_keys(ceil_div(max_length, SOLO_CHUNK), kBlock, max_length, &a.o_splits, &a.o_chunk);
+            } else {
+                split_keys(ceil_div(2 * slots, own), p.own == kWide ? wide_round : round, max_length, &a.o_splits, &a.o_chunk);
+            }
         }
-        if (!own_wide) {
-            while (a.o_tiles > 1 && (int64_t)a.Hkv * a.B * a.o_tiles * (a.o_splits > 0 ? a.o_splits : 1) >= (1 << 22)) a.o_tiles = (a.o_tiles + 1) / 2;
-            return p_wide ? (rt == 2 ? pfr::attn::kMixed2 : pfr::attn::kMixed1) : (rt == 2 ? pfr::attn::kNarrow2 : pfr::attn::kNarrow1);
-        }
+        a.p_tiles = (int32_t)ceil_div(rows, tile(p.prefix));
+        split_keys(ceil_div(slots, (int64_t)a.Hkv * a.p_tiles), p.prefix == kWide ? wide_round : round, a.prefix_len, &a.p_splits,
+                   &a.p_chunk);
+        p.prefix_blocks = (int64_t)a.Hkv * a.p_tiles * a.p_splits;
     }
-    while (a.o_tiles > 1 && (int64_t)a.Hkv * (a.B + 2) * a.o_tiles * (a.o_splits > 0 ? a.o_splits : 1) >= (1 << 22)) a.o_tiles = (a.o_tiles + 1) / 2;
-    return pfr::attn::kWide;
+    if (a.B > 0) {
+        const int64_t each = (int64_t)a.Hkv * (a.B + (a.whole ? 2 : 0)) * (a.o_splits > 0 ? a.o_splits : 1);
+        while (a.o_tiles > 1 && each * a.o_tiles >= (1 << 22)) a.o_tiles = (a.o_tiles + 1) / 2;  // workgroups take several
+        p.own_blocks = a.o_splits > 0 ? ceil_div(each * a.o_tiles, a.solo ? kWaves : 1) : 0;
+    }
+    return p;
+}
+
+void enqueue(pfr_ctx* ctx, const pfr_kv* kv, pfr_dtype dtype, const Args& a, Kind kind, int64_t blocks) {
+    using pfr::attn::launch;
+    if (blocks == 0) return;
+    pfr::require(blocks < (1 << 24), "kv attention: extent too large");
+    hipStream_t s = ctx->stream;
+    if (dtype == PFR_BF16) launch<__bf16, __bf16>(s, a, kind, (unsigned)blocks);
+    else if (dtype == PFR_F16) launch<_Float16, _Float16>(s, a, kind, (unsigned)blocks);
+    else if (kv->dtype == PFR_BF16) launch<float, __bf16>(s, a, kind, (unsigned)blocks);
+    else if (kv->dtype == PFR_F16) launch<float, _Float16>(s, a, kind, (unsigned)blocks);
+    else launch<float, float>(s, a, kind, (unsigned)blocks);
 }
 
 void attention_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* q, pfr_dtype dtype, int64_t T, int64_t heads, int64_t ldq,
@@ -169,9 +207,7 @@ void attention_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* q, pfr_dtype dtyp
     // bounds: what a request may add and hold
     if (max_added == 0 || max_added > T) max_added = T;
     if (max_length == 0 || max_length > room) max_length = room;
-    const Kind kind = plan(ctx->num_cu, dtype != PFR_F32, max_added, max_length, room, a);
-    const int64_t blocks = a.p_items + (int64_t)a.Hkv * (a.B + (a.whole ? 2 : 0)) * a.o_tiles * a.o_splits;
-    pfr::require(blocks < (1 << 24), "kv attention: extent too large");
+    const Plan p = plan(ctx->num_cu, dtype != PFR_F32, max_added, max_length, room, a);
 
     const int64_t parts = a.p_splits + a.o_splits, rows = T * heads;
     if (!a.whole || parts > 1) {
@@ -180,12 +216,12 @@ void attention_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* q, pfr_dtype dtyp
         a.part_o = reinterpret_cast<float*>(ws);
         a.part_ml = reinterpret_cast<float2*>(ws + o);
     }
-    if (blocks > 0) {
-        if (dtype == PFR_BF16) pfr::attn::launch<__bf16, __bf16>(ctx->stream, a, kind, (unsigned)blocks);
-        else if (dtype == PFR_F16) pfr::attn::launch<_Float16, _Float16>(ctx->stream, a, kind, (unsigned)blocks);
-        else if (kv->dtype == PFR_BF16) pfr::attn::launch<float, __bf16>(ctx->stream, a, kind, (unsigned)blocks);
-        else if (kv->dtype == PFR_F16) pfr::attn::launch<float, _Float16>(ctx->stream, a, kind, (unsigned)blocks);
-        else pfr::attn::launch<float, float>(ctx->stream, a, kind, (unsigned)blocks);
+    const bool one = p.prefix == p.own;
+    a.p_items = (int32_t)p.prefix_blocks;
+    enqueue(ctx, kv, dtype, a, p.prefix, p.prefix_blocks + (one ? p.own_blocks : 0));
+    if (!one) {
+        a.p_items = 0;
+        enqueue(ctx, kv, dtype, a, p.own, p.own_blocks);
     }
     if (a.part_o != nullptr) {
         const dim3 grid((unsigned)ceil_div(rows, 4)), wg(256);

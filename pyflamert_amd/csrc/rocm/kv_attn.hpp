@@ -23,6 +23,7 @@ constexpr int kWaves = 4;       // waves of a workgroup
 constexpr int kBlock = 32;      // keys of a wave's block, narrow form
 constexpr int kWideRows = 128;  // rows of a workgroup, wide form: 32 a wave
 constexpr int kWideKeys = 64;   // keys of its tile
+constexpr float kSlack = 8.0f;  // how far (log2) scores may pass the number they are weighed against
 
 struct Args {
     const void* q;
@@ -48,25 +49,26 @@ struct Args {
     int32_t B;
     // Apart: p_items = Hkv * p_tiles * p_splits workgroups for the prefix, p_chunk
     // keys a split, its tiles over the rows of all tokens; then Hkv * B *
-    // o_tiles * o_splits for the requests' own keys, o_chunk a split.
+    // o_tiles * o_splits for the requests' own keys, o_chunk a split, with a
+    // workgroup or (solo) a wave for each.
     // Together (whole): a request's tiles see the prefix and then its own
     // keys; splits are of that whole range.
-    int32_t whole, p_items, p_tiles, p_splits, p_chunk, o_tiles, o_splits, o_chunk;
+    int32_t whole, solo, p_items, p_tiles, p_splits, p_chunk, o_tiles, o_splits, o_chunk;
     float* part_o;    // [p_splits + o_splits][T * Hq][D], null: rows are whole after one workgroup
     float2* part_ml;  // [p_splits + o_splits][T * Hq]: largest score (log2 units), sum of weights
 };
 
-// The kernels of a call: narrow (kNarrow1, 2: 16 or 32 rows, waves share the
-// keys), wide (128 rows, waves share the tile), or the prefix wide and own keys narrow.
-enum Kind { kNarrow1, kNarrow2, kMixed1, kMixed2, kWide };
+// The kernels: narrow (kNarrow1, 2: 16 or 32 rows, waves share the keys) and
+// wide (128 rows, waves share the tile).
+enum Kind { kNarrow1, kNarrow2, kWide };
 
 template <class QT, class KT>
 void launch(hipStream_t s, const Args& a, Kind kind, unsigned blocks);
 
-// Keys [lo, hi) of a table of w entries.
+// Keys [lo, hi) of a table that holds them.
 struct Seg {
     const int32_t* table;
-    int w, lo, hi;
+    int lo, hi;
 };
 
 template <class T>
@@ -199,8 +201,8 @@ struct Tiles {
     // o += V^T p for the lane's eight keys, p in the order of v's registers.
     // With 16-bit products p is rounded to the cache's type (its error, half a
     // step a weight and averaged over the keys, is the size of the output's
-    // own rounding); the sum of the weights keeps 32 bits.
-    __device__ __forceinline__ void add(int rt, const float (&p)[8]) {
+    // own rounding); the sum of the weights keeps 32 bits.  Only where the lane's row is meant (mine).
+    __device__ __forceinline__ void add(int rt, const float (&p)[8], bool mine) {
         if constexpr (kHalf) {
             typename Mfma16<KT>::V8 pv;
 #pragma unroll
@@ -215,20 +217,25 @@ struct Tiles {
                     for (int x = 0; x < 4; ++x)
                         col[x] = __builtin_amdgcn_perm(v[2 * x + 1][c][e / 2], v[2 * x][c][e / 2],
                                                        (e & 1) ? 0x07060302u : 0x05040100u);
-                    o[rt][c * VV + e] = Mfma16<KT>::dot(__builtin_bit_cast(typename Mfma16<KT>::V8, col), pv, o[rt][c * VV + e]);
+                    set(o[rt][c * VV + e], Mfma16<KT>::dot(__builtin_bit_cast(typename Mfma16<KT>::V8, col), pv, o[rt][c * VV + e]), mine);
                 }
         } else {
             typedef KT VK __attribute__((ext_vector_type(VV)));
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int c = 0; c < CC; ++c)
 #pragma unroll
-                for (int c = 0; c < CC; ++c) {
-                    const VK x = __builtin_bit_cast(VK, v[j][c]);
+                for (int e = 0; e < VV; ++e) {
+                    f4 acc = o[rt][c * VV + e];
 #pragma unroll
-                    for (int e = 0; e < VV; ++e)
-                        o[rt][c * VV + e] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x[e], p[j], o[rt][c * VV + e], 0, 0, 0);
+                    for (int j = 0; j < 8; ++j)
+                        acc = __builtin_amdgcn_mfma_f32_16x16x4f32((float)__builtin_bit_cast(VK, v[j][c])[e], p[j], acc, 0, 0, 0);
+                    set(o[rt][c * VV + e], acc, mine);
                 }
         }
+    }
+    static __device__ __forceinline__ void set(f4& o, const f4& x, bool mine) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = mine ? x[i] : o[i];
     }
 };
 
@@ -243,6 +250,13 @@ __device__ __forceinline__ float row_sum(float x) {
 }
 
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// The same number, computed here: what follows from it is not kept in registers
+// across what came before.
+__device__ __forceinline__ int here(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
 
 // Whether four 16-bit values hold an infinity or a NaN.
 template <class T>
@@ -276,11 +290,12 @@ __device__ __forceinline__ s4 read_tr(const char* p) {
 // Writes the rows' part `part`.
 template <class QT, class KT, int DP, int RT, bool FULL>
 __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0, int r0, int n_rows,
-                                       const Seg& seg, int lim0, int per_token, int part) {
+                                       const Seg& seg, int lim0, int per_token, int part, bool solo) {
     const int32_t* __restrict__ table = seg.table;
-    const int table_w = seg.w, lo = seg.lo, hi = seg.hi;
+    const int lo = seg.lo, hi = seg.hi;
     typedef Tiles<QT, KT, DP, RT, FULL> TT;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const int lane = here(threadIdx.x & 63), w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    int n = lane & 15, g = lane >> 4;
     TT x;
     float m[RT], l[RT];
     int lim[RT];
@@ -302,50 +317,68 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
     const KT* kp = static_cast<const KT*>(a.k) + (int64_t)h * a.head_stride;
     const KT* vp = static_cast<const KT*>(a.v) + (int64_t)h * a.head_stride;
 
-    for (int k0 = lo + w * kBlock; k0 < hi; k0 += kWaves * kBlock) {
-        // lane i (and i + 32) finds key i
-        const int key = k0 + (lane & 31);
-        int64_t off = key < hi ? key_offset(a.map, table, table_w, key) : -1;
-        const uint32_t okm = (uint32_t)__ballot(off >= 0);
+    // A block's keys are found two blocks ahead; its K is loaded as soon as the
+    // block before has its scores, its V as soon as that has its sums.
+    const int step = solo ? kBlock : kWaves * kBlock;
+    const int first = solo ? lo : lo + w * kBlock;
+    // lane i (and i + 32) finds key i of a block: its table entry, and once that is there its offset
+    const auto find = [&](int k0) { return key_place(a.map, k0 + (lane & 31), hi); };
+    const auto offset = [&](int k0, const KeyPlace& at, int32_t id) { return key_offset(a.map, at, id, k0 + (lane & 31), hi); };
+    const auto load_k = [&](int64_t off) {
         off = off < 0 ? 0 : off;  // the pool's first row is there to be read
-        if (okm == 0) continue;
 #pragma unroll
         for (int t = 0; t < 2; ++t) x.load_k(t, kp + __shfl((long long)off, 16 * t + n), g, a.D);
+    };
+    const auto load_v = [&](int64_t off) {
+        off = off < 0 ? 0 : off;
 #pragma unroll
         for (int u = 0; u < 8; ++u) x.load_v(u, vp + __shfl((long long)off, (u < 4 ? 0 : 16) + 4 * g + (u & 3)), n, a.D);
-
+    };
+    // No branch around a load: with one, waits for older loads would wait for it too.
+    int64_t off = -1;
+    KeyPlace at1{0, 0};
+    int32_t id1 = 0;
+    if (first < hi) {
+        const KeyPlace at = find(first);
+        const int32_t id = table[at.entry];
+        at1 = find(first + step);
+        id1 = table[at1.entry];
+        off = offset(first, at, id);
+        load_k(off);
+        load_v(off);
+    }
+    for (int k0 = first; k0 < hi; k0 += step) {
+        const int64_t off1 = offset(k0 + step, at1, id1);
+        at1 = find(k0 + 2 * step);
+        id1 = table[at1.entry];
+        const uint32_t okm = (uint32_t)__ballot(off >= 0);
+        f4 sc[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            sc[rt][0] = x.scores(rt, 0);
+            sc[rt][1] = x.scores(rt, 1);
+        }
+        load_k(off1);
         const bool partly = k0 + kBlock > min_lim;
-        uint32_t poison = 0;
         if (okm != ~0u) {
 #pragma unroll
             for (int u = 0; u < 8; ++u)
                 if (!((okm >> ((u < 4 ? 0 : 16) + 4 * g + (u & 3))) & 1)) x.zero_v(u);
         }
+        bool poison = false;
         if (partly) {
-            // A key that only some rows see must not reach the others, and 0
-            // times an infinity or a NaN would: such values are added row by row.
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const uint64_t b = __ballot(x.nonfinite_v(u));
-#pragma unroll
-                for (int gg = 0; gg < 4; ++gg)
-                    if ((b >> (16 * gg)) & 0xffff) poison |= 1u << ((u < 4 ? 0 : 16) + 4 * gg + (u & 3));
-            }
-            if (min_lim > k0) poison &= ~0u << (min_lim - k0);
-            if (poison) {
-#pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    if ((poison >> ((u < 4 ? 0 : 16) + 4 * g + (u & 3))) & 1) x.zero_v(u);
-            }
+            for (int u = 0; u < 8; ++u) poison |= x.nonfinite_v(u);
+            poison = __any(poison);
         }
+        float p[RT][8];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             float s[8];
-            const f4 s0 = x.scores(rt, 0), s1 = x.scores(rt, 1);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                s[i] = s0[i];
-                s[4 + i] = s1[i];
+                s[i] = sc[rt][0][i];
+                s[4 + i] = sc[rt][1][i];
             }
             if (partly || okm != ~0u) {
 #pragma unroll
@@ -357,42 +390,78 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
             float mx = s[0];
 #pragma unroll
             for (int u = 1; u < 8; ++u) mx = fmaxf(mx, s[u]);
-            const float mn = fmaxf(m[rt], row_max(mx) * a.scale), ms = finite_max(mn);
-            const float alpha = __builtin_amdgcn_exp2f(m[rt] - ms);
-            m[rt] = mn;
-            float p[8], sum = 0.0f;
+            const float mn = fmaxf(m[rt], row_max(mx) * a.scale);
+            // m only has to be near the largest score: weights up to 2^kSlack fit every type
+            if (__any(mn > m[rt] + kSlack)) {
+                const float alpha = __builtin_amdgcn_exp2f(m[rt] - finite_max(mn));
+                l[rt] *= alpha;
+#pragma unroll
+                for (int i = 0; i < TT::NT; ++i) x.o[rt][i] *= alpha;
+                m[rt] = mn;
+            }
+            const float ms = finite_max(m[rt]);
+            float sum = 0.0f;
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                p[u] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u], a.scale, -ms));
-                sum = sum + p[u];
+                p[rt][u] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u], a.scale, -ms));
+                sum = sum + p[rt][u];
             }
-            l[rt] = l[rt] * alpha + sum;
+            l[rt] = l[rt] + sum;
+        }
+        if (!poison) {
 #pragma unroll
-            for (int i = 0; i < TT::NT; ++i) x.o[rt][i] *= alpha;
-            x.add(rt, p);
-            for (uint32_t rest = poison; rest; rest &= rest - 1) {
-                const int kk = __builtin_ctz(rest), u0 = (kk >> 4) * 4 + (kk & 3), g0 = (kk >> 2) & 3;
-                float mine = 0.0f;
+            for (int rt = 0; rt < RT; ++rt) x.add(rt, p[rt], true);
+        } else {
+            // A key that only some rows see must not reach the others, and 0 times an
+            // infinity or a NaN would: rows of one limit at a time, the largest
+            // first, with the values past it cleared.
+            for (int cur = INT32_MAX;;) {
+                int next = INT32_MIN;
 #pragma unroll
-                for (int u = 0; u < 8; ++u) mine = u == u0 ? p[u] : mine;
-                const float pk = __shfl(mine, 16 * g0 + n);
-                const KT* row = vp + __shfl((long long)off, kk);
-                if (((okm >> kk) & 1) && k0 + kk < lim[rt]) {
+                for (int rt = 0; rt < RT; ++rt) next = lim[rt] < cur && lim[rt] > next ? lim[rt] : next;
 #pragma unroll
-                    for (int c = 0; c < TT::CC; ++c)
-#pragma unroll
-                        for (int e = 0; e < TT::VV; ++e)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int d = (16 * c + 4 * g + i) * TT::VV + e;
-                                if (FULL || d < a.D) x.o[rt][c * TT::VV + e][i] += pk * (float)row[d];
-                                if (i == 3) __builtin_amdgcn_sched_barrier(0);  // not all of them in registers at once
-                            }
+                for (int o = 8; o; o >>= 1) {
+                    const int y = __shfl_xor(next, o);
+                    next = y > next ? y : next;
                 }
+                cur = __builtin_amdgcn_readfirstlane(next);
+                if (cur == INT32_MIN) break;
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (k0 + (u < 4 ? 0 : 16) + 4 * g + (u & 3) >= cur) x.zero_v(u);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) x.add(rt, p[rt], lim[rt] == cur);
             }
         }
+        load_v(off1);
+        off = off1;
     }
 
+    n = here(n);
+    g = here(g);
+    const int64_t rows_all = (int64_t)a.T * a.Hq;
+    if (solo) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int r = r0 + rt * 16 + n, dt = (int)a.group.div((uint32_t)r);
+            l[rt] = row_sum(l[rt]);
+            if (r >= n_rows) continue;
+            const int64_t at = (int64_t)part * rows_all + (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G);
+            if (g == 0) a.part_ml[at] = make_float2(m[rt], l[rt]);
+#pragma unroll
+            for (int c = 0; c < TT::CC; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < TT::VV; e += 4) {
+                        const int d = (16 * c + 4 * g + i) * TT::VV + e;
+                        if (FULL || d < a.D)
+                            *reinterpret_cast<f4*>(a.part_o + at * a.D + d) =
+                                f4{x.o[rt][c * TT::VV + e][i], x.o[rt][c * TT::VV + e + 1][i], x.o[rt][c * TT::VV + e + 2][i], x.o[rt][c * TT::VV + e + 3][i]};
+                    }
+        }
+        return;
+    }
     // the waves' sums, joined
     float* sm = lds;                       // [kWaves][16 RT] maxima
     float* sl = lds + kWaves * 16 * RT;    // [kWaves][16 RT] sums
@@ -408,7 +477,6 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
         }
     }
     __syncthreads();
-    const int64_t rows_all = (int64_t)a.T * a.Hq;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         if (r0 + rt * 16 >= n_rows) break;
@@ -478,7 +546,7 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
     constexpr int CPR = DP / 8;   // 16-byte chunks of a key's row
     constexpr int LPT = DP / 32;  // chunks of K, and of V, a thread moves per tile
     constexpr int QS = DP / 16, DB = DP / 32, KG = QS / 2;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, n = lane & 31, hh = lane >> 5;
+    const int tid = here(threadIdx.x), lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hh = lane >> 5;
     const int np = (pre.hi - pre.lo + kWideKeys - 1) / kWideKeys;
     const int nt = np + (own.hi - own.lo + kWideKeys - 1) / kWideKeys;
 
@@ -513,11 +581,14 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
     u4 kr[LPT], vr[LPT];
 
     const auto tile_key = [&](int i) { return i < np ? pre.lo + kWideKeys * i : own.lo + kWideKeys * (i - np); };
-    // one wave finds the keys of tile i
-    const auto lookup = [&](int i, int slot) {
+    // lane i finds key i of a tile: its table entry, and once that is there its offset
+    const auto find = [&](int i) {
         const bool p = i < np;
-        const int key = tile_key(i) + lane;
-        const int64_t off = key < (p ? pre.hi : own.hi) ? key_offset(a.map, p ? pre.table : own.table, p ? pre.w : own.w, key) : -1;
+        return key_place(a.map, tile_key(i) + lane, p ? pre.hi : own.hi);
+    };
+    const auto table_of = [&](int i) { return i < np ? pre.table : own.table; };
+    const auto put = [&](int i, int slot, const KeyPlace& at, int32_t id) {
+        const int64_t off = key_offset(a.map, at, id, tile_key(i) + lane, i < np ? pre.hi : own.hi);
         lds.off[slot][lane] = off;
         const unsigned long long ok = __ballot(off >= 0);
         if (lane == 0) lds.ok[slot] = ok;
@@ -566,7 +637,10 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
     };
 
     if (nt > 0) {
-        if (w < 2 && w < nt) lookup(w, w);
+        if (w < 2 && w < nt) {
+            const KeyPlace at = find(w);
+            put(w, w, at, table_of(w)[at.entry]);
+        }
         __syncthreads();
         load(0);
         store(0, 0, 0);
@@ -582,8 +656,12 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
     int slot = 0;
     for (int i = 0; i < nt; ++i) {
         const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot1 == 2 ? 0 : slot1 + 1, buf = i & 1;
-        if (i + 1 < nt) load(slot1);
-        if (i + 2 < nt && w == (i & 3)) lookup(i + 2, slot2);
+        // The table first, so that what needs it does not wait for the rows; and no
+        // branch around a load: with one, waits for older loads would wait for it too.
+        const int i2 = i + 2 < nt ? i + 2 : nt - 1;
+        const KeyPlace at2 = find(i2);
+        const int32_t id2 = table_of(i2)[at2.entry];
+        load(i + 1 < nt ? slot1 : slot);
         const int k0 = tile_key(i);
         const bool mine = i >= np;
         if (wave_valid && (!mine || k0 < wave_max)) {
@@ -624,14 +702,16 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
 #pragma unroll
             for (int x = 0; x < 16; ++x) mx = fmaxf(mx, s[1][x]);
             mx = fmaxf(mx, half_swap(mx));
-            const float mn = fmaxf(m, mx * a.scale), ms = finite_max(mn);
-            if (__any(mn > m)) {
-                const float alpha = __builtin_amdgcn_exp2f(m - ms);
+            const float mn = fmaxf(m, mx * a.scale);
+            // m only has to be near the largest score: weights up to 2^kSlack fit every type
+            if (__any(mn > m + kSlack)) {
+                const float alpha = __builtin_amdgcn_exp2f(m - finite_max(mn));
                 l *= alpha;
 #pragma unroll
                 for (int d = 0; d < DB; ++d) o[d] *= alpha;
                 m = mn;
             }
+            const float ms = finite_max(m);
             V8 p[2][2];
             float sum = 0.0f;
 #pragma unroll
@@ -690,23 +770,26 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
                 }
             }
         }
+        if (i + 2 < nt && w == (i & 3)) put(i2, slot2, at2, id2);
         if (i + 1 < nt) store(i + 1, slot1, buf ^ 1);
         __syncthreads();
         slot = slot1;
     }
 
-    if (!valid) return;
     l = l + half_swap(l);
-    const int64_t R = (int64_t)(t0 + dt) * a.Hq + hq;
+    const int er = r0 + 32 * w + here(n), eh = here(hh);
+    if (er >= n_rows) return;
+    const int edt = (int)a.group.div((uint32_t)er), ehq = h * a.G + er - edt * a.G;
+    const int64_t R = (int64_t)(t0 + edt) * a.Hq + ehq;
     if (part < 0) {
         const float f = l == 0.0f ? 0.0f : 1.0f / l;
         typedef T T4u __attribute__((ext_vector_type(4), aligned(2)));
-        T* row = static_cast<T*>(a.out) + (int64_t)(t0 + dt) * a.ldo + (int64_t)hq * a.D;
+        T* row = static_cast<T*>(a.out) + (int64_t)(t0 + edt) * a.ldo + (int64_t)ehq * a.D;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int c = 32 * d + 8 * j + 4 * hh;
+                const int c = 32 * d + 8 * j + 4 * eh;
                 if (FULL || c < a.D) {
                     T4u x;
 #pragma unroll
@@ -717,13 +800,13 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
         return;
     }
     const int64_t at = (int64_t)part * a.T * a.Hq + R;
-    if (hh == 0) a.part_ml[at] = make_float2(m, l);
+    if (eh == 0) a.part_ml[at] = make_float2(m, l);
     float* row = a.part_o + at * a.D;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int c = 32 * d + 8 * j + 4 * hh;
+            const int c = 32 * d + 8 * j + 4 * eh;
             if (FULL || c < a.D) {
                 f4 x;
 #pragma unroll
@@ -739,6 +822,7 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
 struct Item {
     int h, b, tile, split;  // b < 0: the prefix, for all tokens
 };
+// The prefix's workgroups come first.
 __device__ __forceinline__ Item item_of(const Args& a) {
     int i = (int)blockIdx.x;
     Item x;
@@ -751,6 +835,7 @@ __device__ __forceinline__ Item item_of(const Args& a) {
         return x;
     }
     i -= a.p_items;
+    if (a.solo) i = i * kWaves + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int nb = a.B + (a.whole ? 2 : 0);
     x.h = i % a.Hkv;
     i /= a.Hkv;
@@ -763,18 +848,20 @@ __device__ __forceinline__ Item item_of(const Args& a) {
 
 // No keys for rows [r0, r1) of a part: the join skips what has no weight.
 __device__ __forceinline__ void no_keys(const Args& a, int h, int t0, int r0, int r1, int part) {
-    for (int r = r0 + (int)threadIdx.x; r < r1; r += kWaves * 64) {
+    const int lanes = a.solo && part >= a.p_splits ? 64 : kWaves * 64;
+    for (int r = r0 + ((int)threadIdx.x & (lanes - 1)); r < r1; r += lanes) {
         const int dt = (int)a.group.div((uint32_t)r);
         a.part_ml[(int64_t)part * a.T * a.Hq + (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G)] = make_float2(-INFINITY, 0.0f);
     }
 }
 
-// DN, FULL, RT: the narrow form's; DW, WF: the wide form's (0: there is none);
-// OWN: whether a request's own keys take the wide form too.
-template <class QT, class KT, int DN, bool FULL, int RT, int DW, bool WF, bool OWN>
+// The narrow form (DN columns, FULL: all of them there, RT tiles of rows) or, with
+// DW > 0, the wide one (DW, WF).
+template <class QT, class KT, int DN, bool FULL, int RT, int DW, bool WF>
 __device__ __forceinline__ void attention(const Args& a, char* lds) {
     const Item x = item_of(a);
-    const bool prefix = x.b < 0;
+    if (x.split >= a.o_splits && x.b >= 0) return;  // a wave of its own past the last item
+    const bool prefix = x.b < 0, solo = a.solo && !prefix;
     int t0 = 0, t1 = a.T, lim0 = a.prefix_len, P = a.prefix_len, part = x.split, tiles_apart = a.p_tiles;
     int64_t room = 0;
     const int32_t* table = nullptr;
@@ -794,8 +881,7 @@ __device__ __forceinline__ void attention(const Args& a, char* lds) {
     }
     const int n_rows = (t1 - t0) * a.G;
     const int splits = prefix ? a.p_splits : a.o_splits, chunk = prefix ? a.p_chunk : a.o_chunk;
-    const bool use_wide = OWN || (DW > 0 && prefix);
-    const int rows = use_wide ? kWideRows : 16 * RT;
+    constexpr int rows = DW > 0 ? kWideRows : 16 * RT;
     for (int tile = x.tile; tile * (int64_t)rows < n_rows; tile += tiles_apart) {
         const int r0 = tile * rows, r1 = r0 + rows < n_rows ? r0 + rows : n_rows;
         const int end = prefix ? 0 : keys_end(lim0, (int)a.group.div((uint32_t)(r1 - 1)), room);
@@ -805,17 +891,13 @@ __device__ __forceinline__ void attention(const Args& a, char* lds) {
             no_keys(a, x.h, t0, r0, r1, part);
             continue;
         }
-        const Seg pre{a.prefix_table, INT32_MAX, lo < P ? lo : P, hi < P ? hi : P};
-        const Seg own{table, a.table_w, lo > P ? lo - P : 0, hi > P ? hi - P : 0};
-        if constexpr (OWN) {
+        const Seg pre{a.prefix_table, lo < P ? lo : P, hi < P ? hi : P};
+        const Seg own{table, lo > P ? lo - P : 0, hi > P ? hi - P : 0};
+        if constexpr (DW > 0) {
             wide<QT, DW, WF>(a, *reinterpret_cast<WideLds<DW>*>(lds), x.h, t0, r0, n_rows, pre, own, lim0, part);
-        } else if constexpr (DW > 0) {
-            if (prefix) wide<QT, DW, WF>(a, *reinterpret_cast<WideLds<DW>*>(lds), x.h, t0, r0, n_rows, pre, Seg{nullptr, 0, 0, 0}, 0, part);
-            else narrow<QT, KT, DN, RT, FULL>(a, reinterpret_cast<float*>(lds), x.h, t0, r0, n_rows, own, lim0, 1, part);
-            __syncthreads();
         } else {
-            narrow<QT, KT, DN, RT, FULL>(a, reinterpret_cast<float*>(lds), x.h, t0, r0, n_rows, prefix ? pre : own, lim0, prefix ? 0 : 1, part);
-            __syncthreads();
+            narrow<QT, KT, DN, RT, FULL>(a, reinterpret_cast<float*>(lds), x.h, t0, r0, n_rows, prefix ? pre : own, lim0, prefix ? 0 : 1, part, solo);
+            if (!solo) __syncthreads();
         }
     }
 }
@@ -828,28 +910,19 @@ constexpr int narrow_lds() {
 template <class QT, class KT, int D, bool FULL, int RT>
 __global__ __launch_bounds__(kWaves * 64, RT == 1 && D < 256 ? 2 : 1) void k_attn_narrow(Args a) {
     __shared__ __attribute__((aligned(16))) char lds[narrow_lds<QT, KT, D, FULL, RT>()];
-    attention<QT, KT, D, FULL, RT, 0, false, false>(a, lds);
-}
-
-template <class T, int DN, bool FULL, int RT, int DW, bool WF>
-__global__ __launch_bounds__(kWaves * 64, 2) void k_attn_mixed(Args a) {
-    constexpr int x = narrow_lds<T, T, DN, FULL, RT>(), y = (int)sizeof(WideLds<DW>);
-    __shared__ __attribute__((aligned(16))) char lds[x > y ? x : y];
-    attention<T, T, DN, FULL, RT, DW, WF, false>(a, lds);
+    attention<QT, KT, D, FULL, RT, 0, false>(a, lds);
 }
 
 template <class T, int DW, bool WF>
 __global__ __launch_bounds__(kWaves * 64, 2) void k_attn_wide(Args a) {
     __shared__ __attribute__((aligned(16))) char lds[sizeof(WideLds<DW>)];
-    attention<T, T, 64, false, 1, DW, WF, true>(a, lds);
+    attention<T, T, 64, false, 1, DW, WF>(a, lds);
 }
 
 template <class QT, class KT, int DN, bool FULL, int DW, bool WF>
 void launch_kind(hipStream_t s, const Args& a, Kind kind, unsigned blocks) {
     const dim3 grid(blocks), wg(kWaves * 64);
     if constexpr (DW > 0) {
-        if (kind == kMixed1) { hipLaunchKernelGGL((k_attn_mixed<QT, DN, FULL, 1, DW, WF>), grid, wg, 0, s, a); return; }
-        if (kind == kMixed2) { hipLaunchKernelGGL((k_attn_mixed<QT, DN, FULL, 2, DW, WF>), grid, wg, 0, s, a); return; }
         if (kind == kWide) { hipLaunchKernelGGL((k_attn_wide<QT, DW, WF>), grid, wg, 0, s, a); return; }
     }
     if constexpr (DN < 256) {

@@ -42,14 +42,23 @@ struct PageMap {
     int64_t page_stride = 0, token_stride = 0;
 };
 
-// The offset of a head's row of key `key` (0 <= key < kMaxKeys), -1 where the table
-// (w entries) ends before it or names no page of the pool.
-PFR_HD int64_t key_offset(const PageMap& m, const int32_t* table, int w, int key) {
-    const uint32_t j = m.page.div((uint32_t)key);
-    if (j >= (uint32_t)w) return -1;
-    const int32_t id = table[j];
-    if ((uint32_t)id >= m.pages) return -1;
-    return (int64_t)id * m.page_stride + (int64_t)((uint32_t)key - j * m.page.d) * m.token_stride;
+// Where key `key` of keys [.., hi) stands: the entry of its table (a key past
+// hi takes the last one's, so that a load from the table needs no branch; there
+// is a key below hi, and hi is within what the table holds) and its place in
+// that page.
+struct KeyPlace {
+    uint32_t entry, within;
+};
+PFR_HD KeyPlace key_place(const PageMap& m, int key, int hi) {
+    const uint32_t k = (uint32_t)(key < hi ? key : hi - 1), j = m.page.div(k);
+    return {j, k - j * m.page.d};
+}
+
+// The offset of a head's row of that key with its entry `id`, -1 where the key is
+// past hi or the entry names no page of the pool.
+PFR_HD int64_t key_offset(const PageMap& m, const KeyPlace& p, int32_t id, int key, int hi) {
+    const int64_t off = (int64_t)id * m.page_stride + (int64_t)p.within * m.token_stride;
+    return key < hi && (uint32_t)id < m.pages ? off : -1;
 }
 
 // Tokens [t0, t1) of request b, within the T there are whatever start holds.

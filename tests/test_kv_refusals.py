@@ -179,13 +179,14 @@ int main() {
         m.page_stride = m.token_stride * page + 8 * (r() % 3);
         int32_t* t = (int32_t*)malloc(4 * (w ? w : 1));  // of its size, so that a checker sees a read past it
         for (int i = 0; i < w; ++i) t[i] = (int32_t)(r() % 4 ? r() % 12 : r()) - (r() % 5 == 0 ? 20 : 0);
-        for (int key = 0; key < (w + 2) * page; ++key) {
-            const int64_t o = key_offset(m, t, w, key);
-            const bool in = key / page < w && t[key / page] >= 0 && t[key / page] < (int)m.pages;
+        const int hi = w ? 1 + r() % (w * page) : 0;
+        for (int key = 0; hi && key < (w + 2) * page; ++key) {
+            const KeyPlace p = key_place(m, key, hi);
+            const int64_t o = key_offset(m, p, t[p.entry], key, hi);
+            const bool in = key < hi && t[key / page] >= 0 && t[key / page] < (int)m.pages;
             CHECK((o >= 0) == in);
             if (in) CHECK(o == (int64_t)t[key / page] * m.page_stride + (key % page) * m.token_stride);
         }
-        CHECK(key_offset(m, t, w, kMaxKeys - 1) == -1 || (int64_t)w * page >= kMaxKeys);
         free(t);
     }
     // a pool past 2^32 elements
@@ -195,7 +196,7 @@ int main() {
     big.token_stride = 128;
     big.page_stride = 65536;
     const int32_t far = 2999999;
-    CHECK(key_offset(big, &far, 1, 15) == 2999999ll * 65536 + 15 * 128);
+    CHECK(key_offset(big, key_place(big, 15, 16), far, 15, 16) == 2999999ll * 65536 + 15 * 128);
     // token ranges stay within T for any start
     for (int it = 0; it < 20000; ++it) {
         const int T = r() % 50;
