@@ -161,9 +161,10 @@ struct pfr_ctx {
     // transposed activations of the Gemm form, scratch[4]: the magnitude
     // mask's selection state (histogram, counters, per-block tie counts).
     // scratch[5]: the product before its transpose in the 2:4 x . W form.
-    // scratch[7]: the parts of an attention's rows.
     // scratch[6]: the row and chunk counts of a CSR built on the device.
-    pfr::DevBuf scratch[8];
+    // scratch[7]: the parts of an attention's rows, scratch[8]: their arrival
+    // counters (zero between launches).
+    pfr::DevBuf scratch[9];
     // Page-locked host memory (pfr::kPinnedBytes, allocated on first use) that
     // weight builds send their small tables through; build_mu guards it and
     // scratch[6] (a build that finds them taken uses memory of its own).

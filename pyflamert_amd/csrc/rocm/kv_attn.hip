@@ -11,65 +11,18 @@ namespace {
 
 using pfr::attn::Args;
 using pfr::attn::Kind;
-using pfr::attn::kBlock;
 using pfr::attn::kWaves;
 using pfr::attn::kWideKeys;
 using pfr::attn::kWideRows;
 
-// A wave joins a row: lane p holds part p's statistics, and 32 lanes (64 past 128
-// columns) add up its values, two parts at a time.
+// A wave joins a row, where a launch of its own does that.
 template <class QT>
 __global__ __launch_bounds__(256) void k_kv_attn_join(Args a) {
-    typedef pfr::attn::f4 f4;
-    typedef QT Q4 __attribute__((ext_vector_type(4), aligned(sizeof(QT))));
-    const int lane = threadIdx.x & 63;
     const int64_t rows = (int64_t)a.T * a.Hq, R = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (R >= rows) return;
     const int t = (int)(R / a.Hq);
     const bool own = a.whole || (a.B > 0 && t >= a.start[0] && t < a.start[a.B]);
-    const int parts = a.p_splits + (own ? a.o_splits : 0);
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    if (lane < parts) ml = a.part_ml[lane * rows + R];
-    const bool some = ml.x != -INFINITY || ml.y != 0.0f;
-    const unsigned long long live = __ballot(some);
-    float M = ml.x;
-    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-    const float f = some ? __builtin_amdgcn_exp2f(ml.x - pfr::attn::finite_max(M)) : 0.0f;
-    float L = some ? f * ml.y : 0.0f;
-    for (int o = 32; o; o >>= 1) L = L + __shfl_xor(L, o);
-
-    const bool pair = a.D <= 128;
-    const int step = pair ? 2 : 1, half = pair ? lane >> 5 : 0, d = 4 * (pair ? lane & 31 : lane);
-    const float* src = a.part_o + R * a.D + d;
-    f4 acc = f4(0.0f);
-    constexpr int kAtOnce = 4;
-    for (int p0 = 0; p0 < parts; p0 += step * kAtOnce) {
-        f4 x[kAtOnce];
-        float fp[kAtOnce];
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-            const int p = p0 + i * step + half;
-            fp[i] = __shfl(f, p);
-            const bool there = p < 64 && ((live >> p) & 1) && d < a.D;
-            x[i] = f4(0.0f);
-            if (there) x[i] = *reinterpret_cast<const f4*>(src + p * rows * a.D);
-            else fp[i] = 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = acc[e] + fp[i] * x[i][e];
-    }
-    if (pair) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = acc[e] + __shfl_xor(acc[e], 32);
-    }
-    if (half == 0 && d < a.D) {
-        Q4 x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = (QT)(L == 0.0f ? 0.0f : acc[e] / L);
-        *reinterpret_cast<Q4*>(static_cast<QT*>(a.out) + (int64_t)t * a.ldo + (R - (int64_t)t * a.Hq) * a.D + d) = x;
-    }
+    pfr::attn::join_row<QT, false>(a, R, t, a.p_splits + (own ? a.o_splits : 0));
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -78,6 +31,7 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // about `want` of them, and at most kMaxParts.
 constexpr int kMaxParts = 24;
 #define SOLO_CHUNK 256
+#define JOIN_ROWS 64
 void split_keys(int64_t want, int64_t round, int64_t keys, int32_t* splits, int32_t* chunk) {
     int64_t s = ceil_div(keys, round);
     s = want < s ? want : s;
@@ -94,14 +48,14 @@ struct Plan {
 };
 
 // Which kernels, and how the work is cut into workgroups.
-Plan plan(int num_cu, bool half, int64_t max_added, int64_t max_length, int64_t room, Args& a) {
+Plan plan(int num_cu, bool half,  int64_t max_added, int64_t max_length, int64_t room, Args& a) {
     using namespace pfr::attn;
     Plan p;
     const int64_t rows = (int64_t)a.T * a.G, own_rows = max_added * a.G;  // of a key head
     const auto kind = [&](int64_t n) { return half && a.D <= 128 && n > 32 ? kWide : (a.D <= 128 && n > 16 ? kNarrow2 : kNarrow1); };
     const auto tile = [](Kind k) { return k == kWide ? kWideRows : (k == kNarrow2 ? 32 : 16); };
     const int64_t slots = 2 * num_cu;  // workgroups at a time
-    const int64_t round = kWaves * kBlock, wide_round = 4 * kWideKeys;
+    const int64_t block = half ? kBlock<__bf16> : kBlock<float>, round = kWaves * block, wide_round = 4 * kWideKeys;
 
     p.own = kind(own_rows);
     a.whole = a.B > 0 && p.own == kWide && rows >= 2 * kWideRows * a.B && a.prefix_len + room < INT32_MAX - 4096;
@@ -119,7 +73,7 @@ Plan plan(int num_cu, bool half, int64_t max_added, int64_t max_length, int64_t 
             const int64_t own = (int64_t)a.Hkv * a.B * a.o_tiles;
             if (p.own != kWide && own * ceil_div(max_length, SOLO_CHUNK) >= 2 * kWaves * slots) {
                 a.solo = 1;
-                split_keys(ceil_div(max_length, SOLO_CHUNK), kBlock, max_length, &a.o_splits, &a.o_chunk);
+                split_keys(ceil_div(max_length, SOLO_CHUNK), block, max_length, &a.o_splits, &a.o_chunk);
             } else {
                 split_keys(ceil_div(2 * slots, own), p.own == kWide ? wide_round : round, max_length, &a.o_splits, &a.o_chunk);
             }
@@ -133,6 +87,23 @@ Plan plan(int num_cu, bool half, int64_t max_added, int64_t max_length, int64_t 
         const int64_t each = (int64_t)a.Hkv * (a.B + (a.whole ? 2 : 0)) * (a.o_splits > 0 ? a.o_splits : 1);
         while (a.o_tiles > 1 && each * a.o_tiles >= (1 << 22)) a.o_tiles = (a.o_tiles + 1) / 2;  // workgroups take several
         p.own_blocks = a.o_splits > 0 ? ceil_div(each * a.o_tiles, a.solo ? kWaves : 1) : 0;
+    }
+    return p;
+}
+
+__global__ void k_kv_attn_zero(uint32_t* p, int n) {
+    const int i = (int)(blockIdx.x * blockDim.x + threadIdx.x);
+    if (i < n) p[i] = 0;
+}
+
+// The context's arrival counters, which every launch leaves at zero.
+uint32_t* arrivals(pfr_ctx* ctx, int64_t n) {
+    const size_t had = ctx->scratch[8].bytes, want = (size_t)(n < 16384 ? 16384 : n) * sizeof(uint32_t);
+    auto* p = static_cast<uint32_t*>(ctx->scratch[8].ensure(want));
+    if (ctx->scratch[8].bytes != had) {
+        const int words = (int)(ctx->scratch[8].bytes / sizeof(uint32_t));
+        hipLaunchKernelGGL(k_kv_attn_zero, dim3((unsigned)ceil_div(words, 256)), dim3(256), 0, ctx->stream, p, words);
+        PFR_HIP(hipGetLastError());
     }
     return p;
 }
@@ -217,13 +188,21 @@ void attention_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* q, pfr_dtype dtyp
         a.part_ml = reinterpret_cast<float2*>(ws + o);
     }
     const bool one = p.prefix == p.own;
+    const auto by = [](int64_t n) { return pfr::FastDiv((uint32_t)(n > 0 ? n : 1)); };
+    a.by_heads = by(a.Hkv);
+    a.by_p_tiles = by(a.p_tiles);
+    a.by_o_tiles = by(a.o_tiles);
+    a.by_requests = by(a.B + (a.whole ? 2 : 0));
+    // few enough rows for the workgroups that come last to join them
+    if (one && p.own != pfr::attn::kWide && !a.solo && B > 0 && B + 2 <= 64 && T * a.G <= JOIN_ROWS && p.own_blocks > 0)
+        a.arrived = arrivals(ctx, a.Hkv * (B + 2));
     a.p_items = (int32_t)p.prefix_blocks;
     enqueue(ctx, kv, dtype, a, p.prefix, p.prefix_blocks + (one ? p.own_blocks : 0));
     if (!one) {
         a.p_items = 0;
         enqueue(ctx, kv, dtype, a, p.own, p.own_blocks);
     }
-    if (a.part_o != nullptr) {
+    if (a.part_o != nullptr && a.arrived == nullptr) {
         const dim3 grid((unsigned)ceil_div(rows, 4)), wg(256);
         if (dtype == PFR_BF16) hipLaunchKernelGGL(k_kv_attn_join<__bf16>, grid, wg, 0, ctx->stream, a);
         else if (dtype == PFR_F16) hipLaunchKernelGGL(k_kv_attn_join<_Float16>, grid, wg, 0, ctx->stream, a);

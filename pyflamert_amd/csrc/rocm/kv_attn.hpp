@@ -20,7 +20,10 @@ typedef unsigned u2 __attribute__((ext_vector_type(2)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;       // waves of a workgroup
-constexpr int kBlock = 32;      // keys of a wave's block, narrow form
+// Keys of a wave's block, narrow form: two tiles of 16 make the 32 that a 16-bit
+// product sums over; one keeps a float32 block in registers without spills.
+template <class QT>
+constexpr int kBlock = sizeof(QT) == 2 ? 32 : 16;
 constexpr int kWideRows = 128;  // rows of a workgroup, wide form: 32 a wave
 constexpr int kWideKeys = 64;   // keys of its tile
 constexpr float kSlack = 8.0f;  // how far (log2) scores may pass the number they are weighed against
@@ -53,9 +56,13 @@ struct Args {
     // workgroup or (solo) a wave for each.
     // Together (whole): a request's tiles see the prefix and then its own
     // keys; splits are of that whole range.
+    FastDiv by_heads, by_p_tiles, by_o_tiles, by_requests;
     int32_t whole, solo, p_items, p_tiles, p_splits, p_chunk, o_tiles, o_splits, o_chunk;
     float* part_o;    // [p_splits + o_splits][T * Hq][D], null: rows are whole after one workgroup
-    float2* part_ml;  // [p_splits + o_splits][T * Hq]: largest score (log2 units), sum of weights
+    float2* part_ml;  // [p_splits + o_splits][T * Hq]: the score weighed against (log2 units), sum of weights
+    // Arrivals at each key head's requests (and at the tokens of none), zero
+    // between launches: the last workgroup joins the rows.  Null: a launch of its own does.
+    uint32_t* arrived;  // [Hkv][B + 2]
 };
 
 // The kernels: narrow (kNarrow1, 2: 16 or 32 rows, waves share the keys) and
@@ -124,6 +131,7 @@ __device__ __forceinline__ V signed_q(V q, float sign) {
 template <class QT, class KT, int DP, int RT, bool FULL>
 struct Tiles {
     static constexpr bool kHalf = sizeof(QT) == 2;         // 16-bit products; else float32 ones
+    static constexpr int NK = kBlock<QT> / 16, NJ = 4 * NK;  // key tiles; keys of a lane's values
     static constexpr int VE = 16 / (int)sizeof(KT);         // elements of a 16-byte load
     static constexpr int KS = DP / (4 * VE);                // key loads per lane and tile
     static constexpr int VV = VE < DP / 16 ? VE : DP / 16;  // contiguous values of a lane per load
@@ -135,8 +143,8 @@ struct Tiles {
     typedef KT KV __attribute__((ext_vector_type(VE)));
 
     QV q[RT][KS];
-    KV k[2][KS];
-    VRaw v[8][CC];
+    KV k[NK][KS];
+    VRaw v[NJ][CC];
     f4 o[RT][NT];
 
     // element e of load s of a lane is d = (4 s + g) VE + e, for rows of Q and of K alike
@@ -148,22 +156,23 @@ struct Tiles {
             if (valid && (FULL || d < D)) q[rt][s] = signed_q(QV(*reinterpret_cast<const QVu*>(row + d)), sign);
         }
     }
+    // Past D a lane reads the row's start: no branch around a load.  K is cleared
+    // there when it is used; columns of O there are not stored.
     __device__ __forceinline__ void load_k(int t, const KT* row, int g, int D) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int d = (4 * s + g) * VE;
-            if (FULL || d < D) k[t][s] = *reinterpret_cast<const KV*>(row + d);
-            else k[t][s] = KV(0);
+            k[t][s] = *reinterpret_cast<const KV*>(row + (FULL || d < D ? d : 0));
         }
     }
     // value register j is key 4 g + j of tile 0 (j < 4) or 4 g + j - 4 of tile
     // 1, columns (16 c + n) VV ..
+    static __device__ __forceinline__ int key_of(int j, int g) { return (j < 4 ? 0 : 16) + 4 * g + (j & 3); }
     __device__ __forceinline__ void load_v(int j, const KT* row, int n, int D) {
 #pragma unroll
         for (int c = 0; c < CC; ++c) {
             const int d = (16 * c + n) * VV;
-            if (FULL || d < D) v[j][c] = *reinterpret_cast<const VRaw*>(row + d);
-            else v[j][c] = VRaw(0);
+            v[j][c] = *reinterpret_cast<const VRaw*>(row + (FULL || d < D ? d : 0));
         }
     }
     __device__ __forceinline__ void zero_v(int j) {
@@ -184,25 +193,27 @@ struct Tiles {
             }
         return bad;
     }
-    __device__ __forceinline__ f4 scores(int rt, int t) const {
+    __device__ __forceinline__ f4 scores(int rt, int t, int g, int D) const {
         f4 acc = f4(0.0f);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
+            KV x = k[t][s];
+            if (!FULL && (4 * s + g) * VE >= D) x = KV(0);
             if constexpr (kHalf) {
-                acc = Mfma16<KT>::dot(k[t][s], q[rt][s], acc);
+                acc = Mfma16<KT>::dot(x, q[rt][s], acc);
             } else {
 #pragma unroll
                 for (int e = 0; e < VE; ++e)
-                    acc = __builtin_amdgcn_mfma_f32_16x16x4f32((float)k[t][s][e], q[rt][s][e], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x[e], q[rt][s][e], acc, 0, 0, 0);
             }
         }
         return acc;
     }
-    // o += V^T p for the lane's eight keys, p in the order of v's registers.
+    // o += V^T p for the lane's NJ keys, p in the order of v's registers.
     // With 16-bit products p is rounded to the cache's type (its error, half a
     // step a weight and averaged over the keys, is the size of the output's
     // own rounding); the sum of the weights keeps 32 bits.  Only where the lane's row is meant (mine).
-    __device__ __forceinline__ void add(int rt, const float (&p)[8], bool mine) {
+    __device__ __forceinline__ void add(int rt, const float (&p)[NJ], bool mine) {
         if constexpr (kHalf) {
             typename Mfma16<KT>::V8 pv;
 #pragma unroll
@@ -227,7 +238,7 @@ struct Tiles {
                 for (int e = 0; e < VV; ++e) {
                     f4 acc = o[rt][c * VV + e];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
+                    for (int j = 0; j < NJ; ++j)
                         acc = __builtin_amdgcn_mfma_f32_16x16x4f32((float)__builtin_bit_cast(VK, v[j][c])[e], p[j], acc, 0, 0, 0);
                     set(o[rt][c * VV + e], acc, mine);
                 }
@@ -278,6 +289,78 @@ __device__ __forceinline__ float half_swap(float x) {
     return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
 }
 
+// Two floats to and from memory that workgroups share within a launch: device-
+// scope (agent) atomics, which the hardware keeps coherent across the XCDs' L2
+// caches; a fence would write back and invalidate the whole L2 instead.
+__device__ __forceinline__ void put_pair(float2* p, float x, float y) {
+    const unsigned long long v = (unsigned long long)__builtin_bit_cast(unsigned, y) << 32 | __builtin_bit_cast(unsigned, x);
+    __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get_pair(const float2* p) {
+    const unsigned long long v =
+        __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__builtin_bit_cast(float, (unsigned)v), __builtin_bit_cast(float, (unsigned)(v >> 32)));
+}
+
+// A wave joins the parts of row R (query head R % Hq of token t): lane p holds part
+// p's statistics, and 32 lanes (64 past 128 columns) add up its values, two
+// parts at a time.  SHARED: the parts are of this launch.
+template <class QT, bool SHARED>
+__device__ __forceinline__ void join_row(const Args& a, int64_t R, int t, int parts) {
+    typedef QT Q4 __attribute__((ext_vector_type(4), aligned(sizeof(QT))));
+    const int lane = threadIdx.x & 63;
+    const int64_t rows = (int64_t)a.T * a.Hq;
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (lane < parts) ml = SHARED ? get_pair(a.part_ml + lane * rows + R) : a.part_ml[lane * rows + R];
+    const bool some = ml.x != -INFINITY || ml.y != 0.0f;
+    const unsigned long long live = __ballot(some);
+    float M = ml.x;
+    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+    const float f = some ? __builtin_amdgcn_exp2f(ml.x - finite_max(M)) : 0.0f;
+    float L = some ? f * ml.y : 0.0f;
+    for (int o = 32; o; o >>= 1) L = L + __shfl_xor(L, o);
+
+    const bool pair = a.D <= 128;
+    const int step = pair ? 2 : 1, half = pair ? lane >> 5 : 0, d = 4 * (pair ? lane & 31 : lane);
+    const float* src = a.part_o + R * a.D + d;
+    f4 acc = f4(0.0f);
+    constexpr int kAtOnce = 4;
+    for (int p0 = 0; p0 < parts; p0 += step * kAtOnce) {
+        f4 x[kAtOnce];
+        float fp[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int p = p0 + i * step + half;
+            fp[i] = __shfl(f, p);
+            const bool there = p < 64 && ((live >> p) & 1) && d < a.D;
+            x[i] = f4(0.0f);
+            if (!there) {
+                fp[i] = 0.0f;
+            } else if (SHARED) {
+                const float2* at = reinterpret_cast<const float2*>(src + p * rows * a.D);
+                const float2 u = get_pair(at), v = get_pair(at + 1);
+                x[i] = f4{u.x, u.y, v.x, v.y};
+            } else {
+                x[i] = *reinterpret_cast<const f4*>(src + p * rows * a.D);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = acc[e] + fp[i] * x[i][e];
+    }
+    if (pair) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = acc[e] + __shfl_xor(acc[e], 32);
+    }
+    if (half == 0 && d < a.D) {
+        Q4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = (QT)(L == 0.0f ? 0.0f : acc[e] / L);
+        *reinterpret_cast<Q4*>(static_cast<QT*>(a.out) + (int64_t)t * a.ldo + (R - (int64_t)t * a.Hq) * a.D + d) = x;
+    }
+}
+
 // Four 16-bit elements a lane of a tile in the LDS, transposed among 16 lanes:
 // lane i gets element i % 4 of what lanes i / 4, i / 4 + 4, .. + 12 address.
 __device__ __forceinline__ s4 read_tr(const char* p) {
@@ -319,20 +402,21 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
 
     // A block's keys are found two blocks ahead; its K is loaded as soon as the
     // block before has its scores, its V as soon as that has its sums.
-    const int step = solo ? kBlock : kWaves * kBlock;
-    const int first = solo ? lo : lo + w * kBlock;
-    // lane i (and i + 32) finds key i of a block: its table entry, and once that is there its offset
-    const auto find = [&](int k0) { return key_place(a.map, k0 + (lane & 31), hi); };
-    const auto offset = [&](int k0, const KeyPlace& at, int32_t id) { return key_offset(a.map, at, id, k0 + (lane & 31), hi); };
+    // lane i (modulo a block) finds key i of a block: its table entry, and once that is there its offset
+    constexpr int kB = kBlock<QT>, NJ = TT::NJ;
+    constexpr uint32_t kAll = kB == 32 ? ~0u : (1u << kB) - 1;
+    const int step = solo ? kB : kWaves * kB, first = solo ? lo : lo + w * kB;
+    const auto find = [&](int k0) { return key_place(a.map, k0 + (lane & (kB - 1)), hi); };
+    const auto offset = [&](int k0, const KeyPlace& at, int32_t id) { return key_offset(a.map, at, id, k0 + (lane & (kB - 1)), hi); };
     const auto load_k = [&](int64_t off) {
         off = off < 0 ? 0 : off;  // the pool's first row is there to be read
 #pragma unroll
-        for (int t = 0; t < 2; ++t) x.load_k(t, kp + __shfl((long long)off, 16 * t + n), g, a.D);
+        for (int t = 0; t < TT::NK; ++t) x.load_k(t, kp + __shfl((long long)off, 16 * t + n), g, a.D);
     };
     const auto load_v = [&](int64_t off) {
         off = off < 0 ? 0 : off;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) x.load_v(u, vp + __shfl((long long)off, (u < 4 ? 0 : 16) + 4 * g + (u & 3)), n, a.D);
+        for (int u = 0; u < NJ; ++u) x.load_v(u, vp + __shfl((long long)off, TT::key_of(u, g)), n, a.D);
     };
     // No branch around a load: with one, waits for older loads would wait for it too.
     int64_t off = -1;
@@ -351,45 +435,40 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
         const int64_t off1 = offset(k0 + step, at1, id1);
         at1 = find(k0 + 2 * step);
         id1 = table[at1.entry];
-        const uint32_t okm = (uint32_t)__ballot(off >= 0);
-        f4 sc[RT][2];
+        const uint32_t okm = (uint32_t)__ballot(off >= 0) & kAll;
+        float p[RT][NJ];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            sc[rt][0] = x.scores(rt, 0);
-            sc[rt][1] = x.scores(rt, 1);
-        }
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int t = 0; t < TT::NK; ++t) {
+                const f4 sc = x.scores(rt, t, g, a.D);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[rt][4 * t + i] = sc[i];
+            }
         load_k(off1);
-        const bool partly = k0 + kBlock > min_lim;
-        if (okm != ~0u) {
+        const bool partly = k0 + kB > min_lim;
+        if (okm != kAll) {
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (!((okm >> ((u < 4 ? 0 : 16) + 4 * g + (u & 3))) & 1)) x.zero_v(u);
+            for (int u = 0; u < NJ; ++u)
+                if (!((okm >> TT::key_of(u, g)) & 1)) x.zero_v(u);
         }
         bool poison = false;
         if (partly) {
 #pragma unroll
-            for (int u = 0; u < 8; ++u) poison |= x.nonfinite_v(u);
+            for (int u = 0; u < NJ; ++u) poison |= x.nonfinite_v(u);
             poison = __any(poison);
         }
-        float p[RT][8];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            float s[8];
+            if (partly || okm != kAll) {
+                const int see = lim[rt] - k0;
+                const uint32_t there = (okm & (see >= 32 ? ~0u : (see <= 0 ? 0u : (1u << see) - 1))) >> (4 * g);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[i] = sc[rt][0][i];
-                s[4 + i] = sc[rt][1][i];
+                for (int u = 0; u < NJ; ++u) p[rt][u] = there & (1u << TT::key_of(u, 0)) ? p[rt][u] : -INFINITY;
             }
-            if (partly || okm != ~0u) {
+            float mx = p[rt][0];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int kk = (u < 4 ? 0 : 16) + 4 * g + (u & 3);
-                    if (!((okm >> kk) & 1) || k0 + kk >= lim[rt]) s[u] = -INFINITY;
-                }
-            }
-            float mx = s[0];
-#pragma unroll
-            for (int u = 1; u < 8; ++u) mx = fmaxf(mx, s[u]);
+            for (int u = 1; u < NJ; ++u) mx = fmaxf(mx, p[rt][u]);
             const float mn = fmaxf(m[rt], row_max(mx) * a.scale);
             // m only has to be near the largest score: weights up to 2^kSlack fit every type
             if (__any(mn > m[rt] + kSlack)) {
@@ -402,8 +481,8 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
             const float ms = finite_max(m[rt]);
             float sum = 0.0f;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                p[rt][u] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u], a.scale, -ms));
+            for (int u = 0; u < NJ; ++u) {
+                p[rt][u] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[rt][u], a.scale, -ms));
                 sum = sum + p[rt][u];
             }
             l[rt] = l[rt] + sum;
@@ -427,8 +506,8 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
                 cur = __builtin_amdgcn_readfirstlane(next);
                 if (cur == INT32_MIN) break;
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    if (k0 + (u < 4 ? 0 : 16) + 4 * g + (u & 3) >= cur) x.zero_v(u);
+                for (int u = 0; u < NJ; ++u)
+                    if (k0 + TT::key_of(u, g) >= cur) x.zero_v(u);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) x.add(rt, p[rt], lim[rt] == cur);
             }
@@ -491,7 +570,7 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
                 L = L + sl[i * 16 * RT + rt * 16 + n] * __builtin_amdgcn_exp2f(sm[i * 16 * RT + rt * 16 + n] - finite_max(M));
             const int r = r0 + rt * 16 + n, dt = (int)a.group.div((uint32_t)r);
             const int64_t R = (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G);
-            a.part_ml[(int64_t)part * rows_all + R] = make_float2(M, L);
+            put_pair(a.part_ml + (int64_t)part * rows_all + R, M, L);
         }
 #pragma unroll
         for (int c = 0; c < TT::CC; ++c) {
@@ -501,15 +580,19 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mine[(4 * g + i) * TT::VV + e] = x.o[rt][c * TT::VV + e][i] * f;
             __syncthreads();
-            for (int z = threadIdx.x; z < 16 * kCols; z += kWaves * 64) {
-                const int rr = z / kCols, cc = z % kCols, r = r0 + rt * 16 + rr, d = c * kCols + cc;
-                if (r < n_rows && d < a.D) {
-                    float sum = 0.0f;
+            for (int z = threadIdx.x; z < 16 * kCols / 2; z += kWaves * 64) {
+                const int rr = z / (kCols / 2), cc = 2 * (z % (kCols / 2)), r = r0 + rt * 16 + rr, d = c * kCols + cc;
+                if (r < n_rows && (FULL || d < a.D)) {
+                    float sx = 0.0f, sy = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < kWaves; ++i) sum = sum + so[i * 16 * kPitch + rr * kPitch + cc];
+                    for (int i = 0; i < kWaves; ++i) {
+                        const float2 y = *reinterpret_cast<const float2*>(so + i * 16 * kPitch + rr * kPitch + cc);
+                        sx = sx + y.x;
+                        sy = sy + y.y;
+                    }
                     const int dt = (int)a.group.div((uint32_t)r);
                     const int64_t R = (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G);
-                    a.part_o[((int64_t)part * rows_all + R) * a.D + d] = sum;
+                    put_pair(reinterpret_cast<float2*>(a.part_o + ((int64_t)part * rows_all + R) * a.D + d), sx, sy);
                 }
             }
             __syncthreads();
@@ -824,25 +907,26 @@ struct Item {
 };
 // The prefix's workgroups come first.
 __device__ __forceinline__ Item item_of(const Args& a) {
-    int i = (int)blockIdx.x;
+    uint32_t i = blockIdx.x;
     Item x;
-    if (i < a.p_items) {
-        x.h = i % a.Hkv;
-        i /= a.Hkv;
+    const auto next = [&i](const FastDiv& f) {
+        const uint32_t q = f.div(i), r = i - q * f.d;
+        i = q;
+        return (int)r;
+    };
+    if (i < (uint32_t)a.p_items) {
+        x.h = next(a.by_heads);
         x.b = -1;
-        x.tile = i % a.p_tiles;
-        x.split = i / a.p_tiles;
+        x.tile = next(a.by_p_tiles);
+        x.split = (int)i;
         return x;
     }
     i -= a.p_items;
     if (a.solo) i = i * kWaves + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int nb = a.B + (a.whole ? 2 : 0);
-    x.h = i % a.Hkv;
-    i /= a.Hkv;
-    x.tile = i % a.o_tiles;
-    i /= a.o_tiles;
-    x.b = i % nb;
-    x.split = i / nb;
+    x.h = next(a.by_heads);
+    x.tile = next(a.by_o_tiles);
+    x.b = next(a.by_requests);
+    x.split = (int)i;
     return x;
 }
 
@@ -851,8 +935,47 @@ __device__ __forceinline__ void no_keys(const Args& a, int h, int t0, int r0, in
     const int lanes = a.solo && part >= a.p_splits ? 64 : kWaves * 64;
     for (int r = r0 + ((int)threadIdx.x & (lanes - 1)); r < r1; r += lanes) {
         const int dt = (int)a.group.div((uint32_t)r);
-        a.part_ml[(int64_t)part * a.T * a.Hq + (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G)] = make_float2(-INFINITY, 0.0f);
+        put_pair(a.part_ml + (int64_t)part * a.T * a.Hq + (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G), -INFINITY, 0.0f);
     }
+}
+
+// A workgroup joins the rows of request b, or of the tokens of none (b = B, B + 1).
+template <class QT>
+__device__ __forceinline__ void join_rows(const Args& a, int h, int b) {
+    int t0, t1;
+    tokens_of(a.start, a.B, b, a.T, &t0, &t1);
+    const int parts = a.p_splits + (b < a.B ? a.o_splits : 0);
+    for (int r = (int)threadIdx.x >> 6; r < (t1 - t0) * a.G; r += kWaves) {
+        const int dt = (int)a.group.div((uint32_t)r);
+        join_row<QT, true>(a, (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G), t0 + dt, parts);
+    }
+}
+
+// A workgroup has written its part of the rows of request b (b < 0: of all
+// tokens).  Where it is the last of those that have a part in a request's
+// rows, it joins them.  Nothing waits: whoever comes last does the work, and
+// the sum does not depend on who that is.
+template <class QT>
+__device__ __forceinline__ void arrive(const Args& a, int h, int b, unsigned long long* flags) {
+    __builtin_amdgcn_s_waitcnt(0);  // the wave's stores have reached their coherent home
+    __syncthreads();
+    const int lane = threadIdx.x & 63, w = (int)threadIdx.x >> 6;
+    if (w == 0) {
+        // lane i: request i, or the tokens of none (B, B + 1); up to 64 of them
+        bool last = false;
+        if (b < 0 ? lane < a.B + 2 : lane == b) {
+            int t0, t1;
+            tokens_of(a.start, a.B, lane, a.T, &t0, &t1);
+            const uint32_t all = a.p_tiles * a.p_splits + (lane < a.B ? a.o_tiles * a.o_splits : 0);
+            uint32_t* at = a.arrived + h * (a.B + 2) + lane;
+            last = t1 > t0 && __hip_atomic_fetch_add(at, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == all;
+            if (last) __hip_atomic_store(at, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        const unsigned long long mask = __ballot(last);
+        if (lane == 0) *flags = mask;
+    }
+    __syncthreads();
+    for (unsigned long long mask = uniform(*flags); mask; mask &= mask - 1) join_rows<QT>(a, h, __builtin_ctzll(mask));
 }
 
 // The narrow form (DN columns, FULL: all of them there, RT tiles of rows) or, with
@@ -898,6 +1021,14 @@ __device__ __forceinline__ void attention(const Args& a, char* lds) {
         } else {
             narrow<QT, KT, DN, RT, FULL>(a, reinterpret_cast<float*>(lds), x.h, t0, r0, n_rows, prefix ? pre : own, lim0, prefix ? 0 : 1, part, solo);
             if (!solo) __syncthreads();
+        }
+    }
+    if constexpr (DW == 0) {
+        if (a.arrived != nullptr) {
+            if (n_rows > 0) arrive<QT>(a, x.h, x.b, reinterpret_cast<unsigned long long*>(lds));
+            // without a prefix nothing else comes to the tokens of no request
+            if (a.p_splits == 0 && x.b == 0 && x.tile == 0 && x.split == 0)
+                for (int b = a.B; b < a.B + 2; ++b) join_rows<QT>(a, x.h, b);
         }
     }
 }
