@@ -30,8 +30,9 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Splits of `keys` keys, each of `chunk` keys (a multiple of `round`), for
 // about `want` of them, and at most kMaxParts.
 constexpr int kMaxParts = 24;
-#define SOLO_CHUNK 256
-#define JOIN_ROWS 64
+#ifndef EV
+#define EV(n, d) d
+#endif
 void split_keys(int64_t want, int64_t round, int64_t keys, int32_t* splits, int32_t* chunk) {
     int64_t s = ceil_div(keys, round);
     s = want < s ? want : s;
@@ -45,6 +46,7 @@ void split_keys(int64_t want, int64_t round, int64_t keys, int32_t* splits, int3
 struct Plan {
     Kind prefix = pfr::attn::kNarrow1, own = pfr::attn::kNarrow1;
     int64_t prefix_blocks = 0, own_blocks = 0;
+    bool mixed = false;  // the prefix wide, own keys narrow
 };
 
 // Which kernels, and how the work is cut into workgroups.
@@ -66,27 +68,33 @@ Plan plan(int num_cu, bool half,  int64_t max_added, int64_t max_length, int64_t
         if (a.o_splits == 0) a.o_splits = 1;
     } else {
         p.prefix = kind(rows);
-        if (a.B > 0) {
-            // one kernel for both where it costs no more than half of its rows
-            if (p.prefix != kWide && p.own != kWide) p.prefix = p.own = p.prefix > p.own ? p.prefix : p.own;
-            a.o_tiles = (int32_t)ceil_div(own_rows, tile(p.own));
-            const int64_t own = (int64_t)a.Hkv * a.B * a.o_tiles;
-            if (p.own != kWide && own * ceil_div(max_length, SOLO_CHUNK) >= 2 * kWaves * slots) {
-                a.solo = 1;
-                split_keys(ceil_div(max_length, SOLO_CHUNK), block, max_length, &a.o_splits, &a.o_chunk);
-            } else {
-                split_keys(ceil_div(2 * slots, own), p.own == kWide ? wide_round : round, max_length, &a.o_splits, &a.o_chunk);
-            }
-        }
+        if (a.B > 0 && p.prefix != kWide && p.own != kWide) p.prefix = p.own = p.prefix > p.own ? p.prefix : p.own;
         a.p_tiles = (int32_t)ceil_div(rows, tile(p.prefix));
-        split_keys(ceil_div(slots, (int64_t)a.Hkv * a.p_tiles), p.prefix == kWide ? wide_round : round, a.prefix_len, &a.p_splits,
-                   &a.p_chunk);
+        a.o_tiles = a.B > 0 ? (int32_t)ceil_div(own_rows, tile(p.own)) : 0;
+        const int64_t prefix_items = (int64_t)a.Hkv * a.p_tiles, own_items = (int64_t)a.Hkv * a.B * a.o_tiles;
+        if (p.prefix != kWide && p.own != kWide) {
+            // chunks of one size, four workgroups to a CU if all requests were of max_length
+            const int64_t keys = prefix_items * a.prefix_len + own_items * max_length;
+            const int64_t c = ceil_div(ceil_div(keys, 2 * slots), round) * round;
+            split_keys(ceil_div(a.prefix_len, c), round, a.prefix_len, &a.p_splits, &a.p_chunk);
+            split_keys(ceil_div(max_length, c), round, max_length, &a.o_splits, &a.o_chunk);
+        } else {
+            if (EV("X_MIX", 1) && p.own != kWide && own_items > 0) {
+                // the prefix's workgroups, bound by their products, share the CUs with the requests', bound by memory
+                p.mixed = true;
+                split_keys(ceil_div(num_cu * EV("X_P", 100) / 100, prefix_items), wide_round, a.prefix_len, &a.p_splits, &a.p_chunk);
+            } else {
+                split_keys(ceil_div(slots, prefix_items), wide_round, a.prefix_len, &a.p_splits, &a.p_chunk);
+            }
+            if (a.B > 0)
+                split_keys(ceil_div(EV("X_O", 2) * slots, own_items), p.own == kWide ? wide_round : round, max_length, &a.o_splits, &a.o_chunk);
+        }
         p.prefix_blocks = (int64_t)a.Hkv * a.p_tiles * a.p_splits;
     }
     if (a.B > 0) {
         const int64_t each = (int64_t)a.Hkv * (a.B + (a.whole ? 2 : 0)) * (a.o_splits > 0 ? a.o_splits : 1);
         while (a.o_tiles > 1 && each * a.o_tiles >= (1 << 22)) a.o_tiles = (a.o_tiles + 1) / 2;  // workgroups take several
-        p.own_blocks = a.o_splits > 0 ? ceil_div(each * a.o_tiles, a.solo ? kWaves : 1) : 0;
+        p.own_blocks = a.o_splits > 0 ? each * a.o_tiles : 0;
     }
     return p;
 }
@@ -187,17 +195,19 @@ void attention_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* q, pfr_dtype dtyp
         a.part_o = reinterpret_cast<float*>(ws);
         a.part_ml = reinterpret_cast<float2*>(ws + o);
     }
-    const bool one = p.prefix == p.own;
+    const bool one = p.mixed || p.prefix == p.own;
     const auto by = [](int64_t n) { return pfr::FastDiv((uint32_t)(n > 0 ? n : 1)); };
     a.by_heads = by(a.Hkv);
     a.by_p_tiles = by(a.p_tiles);
     a.by_o_tiles = by(a.o_tiles);
     a.by_requests = by(a.B + (a.whole ? 2 : 0));
-    // few enough rows for the workgroups that come last to join them
-    if (one && p.own != pfr::attn::kWide && !a.solo && B > 0 && B + 2 <= 64 && T * a.G <= JOIN_ROWS && p.own_blocks > 0)
+    // the workgroups that come last join the rows, where few enough requests share the prefix's
+    if (a.part_o != nullptr && p.own != pfr::attn::kWide && p.own_blocks > 0 &&
+        (!one || (!p.mixed && B + 2 <= 64 && T * a.G <= 64)))
         a.arrived = arrivals(ctx, a.Hkv * (B + 2));
     a.p_items = (int32_t)p.prefix_blocks;
-    enqueue(ctx, kv, dtype, a, p.prefix, p.prefix_blocks + (one ? p.own_blocks : 0));
+    const Kind kind = p.mixed ? (p.own == pfr::attn::kNarrow2 ? pfr::attn::kMixed2 : pfr::attn::kMixed1) : p.prefix;
+    enqueue(ctx, kv, dtype, a, kind, p.prefix_blocks + (one ? p.own_blocks : 0));
     if (!one) {
         a.p_items = 0;
         enqueue(ctx, kv, dtype, a, p.own, p.own_blocks);

@@ -52,12 +52,11 @@ struct Args {
     int32_t B;
     // Apart: p_items = Hkv * p_tiles * p_splits workgroups for the prefix, p_chunk
     // keys a split, its tiles over the rows of all tokens; then Hkv * B *
-    // o_tiles * o_splits for the requests' own keys, o_chunk a split, with a
-    // workgroup or (solo) a wave for each.
+    // o_tiles * o_splits for the requests' own keys, o_chunk a split.
     // Together (whole): a request's tiles see the prefix and then its own
     // keys; splits are of that whole range.
     FastDiv by_heads, by_p_tiles, by_o_tiles, by_requests;
-    int32_t whole, solo, p_items, p_tiles, p_splits, p_chunk, o_tiles, o_splits, o_chunk;
+    int32_t whole, p_items, p_tiles, p_splits, p_chunk, o_tiles, o_splits, o_chunk;
     float* part_o;    // [p_splits + o_splits][T * Hq][D], null: rows are whole after one workgroup
     float2* part_ml;  // [p_splits + o_splits][T * Hq]: the score weighed against (log2 units), sum of weights
     // Arrivals at each key head's requests (and at the tokens of none), zero
@@ -66,8 +65,8 @@ struct Args {
 };
 
 // The kernels: narrow (kNarrow1, 2: 16 or 32 rows, waves share the keys) and
-// wide (128 rows, waves share the tile).
-enum Kind { kNarrow1, kNarrow2, kWide };
+// wide (128 rows, waves share the tile); mixed: the prefix wide, own keys narrow.
+enum Kind { kNarrow1, kNarrow2, kWide, kMixed1, kMixed2 };
 
 template <class QT, class KT>
 void launch(hipStream_t s, const Args& a, Kind kind, unsigned blocks);
@@ -373,7 +372,7 @@ __device__ __forceinline__ s4 read_tr(const char* p) {
 // Writes the rows' part `part`.
 template <class QT, class KT, int DP, int RT, bool FULL>
 __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0, int r0, int n_rows,
-                                       const Seg& seg, int lim0, int per_token, int part, bool solo) {
+                                       const Seg& seg, int lim0, int per_token, int part) {
     const int32_t* __restrict__ table = seg.table;
     const int lo = seg.lo, hi = seg.hi;
     typedef Tiles<QT, KT, DP, RT, FULL> TT;
@@ -405,7 +404,8 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
     // lane i (modulo a block) finds key i of a block: its table entry, and once that is there its offset
     constexpr int kB = kBlock<QT>, NJ = TT::NJ;
     constexpr uint32_t kAll = kB == 32 ? ~0u : (1u << kB) - 1;
-    const int step = solo ? kB : kWaves * kB, first = solo ? lo : lo + w * kB;
+    constexpr int step = kWaves * kB;
+    const int first = lo + w * kB;
     const auto find = [&](int k0) { return key_place(a.map, k0 + (lane & (kB - 1)), hi); };
     const auto offset = [&](int k0, const KeyPlace& at, int32_t id) { return key_offset(a.map, at, id, k0 + (lane & (kB - 1)), hi); };
     const auto load_k = [&](int64_t off) {
@@ -519,28 +519,6 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
     n = here(n);
     g = here(g);
     const int64_t rows_all = (int64_t)a.T * a.Hq;
-    if (solo) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const int r = r0 + rt * 16 + n, dt = (int)a.group.div((uint32_t)r);
-            l[rt] = row_sum(l[rt]);
-            if (r >= n_rows) continue;
-            const int64_t at = (int64_t)part * rows_all + (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G);
-            if (g == 0) a.part_ml[at] = make_float2(m[rt], l[rt]);
-#pragma unroll
-            for (int c = 0; c < TT::CC; ++c)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < TT::VV; e += 4) {
-                        const int d = (16 * c + 4 * g + i) * TT::VV + e;
-                        if (FULL || d < a.D)
-                            *reinterpret_cast<f4*>(a.part_o + at * a.D + d) =
-                                f4{x.o[rt][c * TT::VV + e][i], x.o[rt][c * TT::VV + e + 1][i], x.o[rt][c * TT::VV + e + 2][i], x.o[rt][c * TT::VV + e + 3][i]};
-                    }
-        }
-        return;
-    }
     // the waves' sums, joined
     float* sm = lds;                       // [kWaves][16 RT] maxima
     float* sl = lds + kWaves * 16 * RT;    // [kWaves][16 RT] sums
@@ -922,7 +900,6 @@ __device__ __forceinline__ Item item_of(const Args& a) {
         return x;
     }
     i -= a.p_items;
-    if (a.solo) i = i * kWaves + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     x.h = next(a.by_heads);
     x.tile = next(a.by_o_tiles);
     x.b = next(a.by_requests);
@@ -932,8 +909,7 @@ __device__ __forceinline__ Item item_of(const Args& a) {
 
 // No keys for rows [r0, r1) of a part: the join skips what has no weight.
 __device__ __forceinline__ void no_keys(const Args& a, int h, int t0, int r0, int r1, int part) {
-    const int lanes = a.solo && part >= a.p_splits ? 64 : kWaves * 64;
-    for (int r = r0 + ((int)threadIdx.x & (lanes - 1)); r < r1; r += lanes) {
+    for (int r = r0 + (int)threadIdx.x; r < r1; r += kWaves * 64) {
         const int dt = (int)a.group.div((uint32_t)r);
         put_pair(a.part_ml + (int64_t)part * a.T * a.Hq + (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G), -INFINITY, 0.0f);
     }
@@ -966,7 +942,7 @@ __device__ __forceinline__ void arrive(const Args& a, int h, int b, unsigned lon
         if (b < 0 ? lane < a.B + 2 : lane == b) {
             int t0, t1;
             tokens_of(a.start, a.B, lane, a.T, &t0, &t1);
-            const uint32_t all = a.p_tiles * a.p_splits + (lane < a.B ? a.o_tiles * a.o_splits : 0);
+            const uint32_t all = (a.p_items > 0 ? a.p_tiles * a.p_splits : 0) + (lane < a.B ? a.o_tiles * a.o_splits : 0);
             uint32_t* at = a.arrived + h * (a.B + 2) + lane;
             last = t1 > t0 && __hip_atomic_fetch_add(at, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == all;
             if (last) __hip_atomic_store(at, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -983,8 +959,7 @@ __device__ __forceinline__ void arrive(const Args& a, int h, int b, unsigned lon
 template <class QT, class KT, int DN, bool FULL, int RT, int DW, bool WF>
 __device__ __forceinline__ void attention(const Args& a, char* lds) {
     const Item x = item_of(a);
-    if (x.split >= a.o_splits && x.b >= 0) return;  // a wave of its own past the last item
-    const bool prefix = x.b < 0, solo = a.solo && !prefix;
+    const bool prefix = x.b < 0;
     int t0 = 0, t1 = a.T, lim0 = a.prefix_len, P = a.prefix_len, part = x.split, tiles_apart = a.p_tiles;
     int64_t room = 0;
     const int32_t* table = nullptr;
@@ -1019,8 +994,8 @@ __device__ __forceinline__ void attention(const Args& a, char* lds) {
         if constexpr (DW > 0) {
             wide<QT, DW, WF>(a, *reinterpret_cast<WideLds<DW>*>(lds), x.h, t0, r0, n_rows, pre, own, lim0, part);
         } else {
-            narrow<QT, KT, DN, RT, FULL>(a, reinterpret_cast<float*>(lds), x.h, t0, r0, n_rows, prefix ? pre : own, lim0, prefix ? 0 : 1, part, solo);
-            if (!solo) __syncthreads();
+            narrow<QT, KT, DN, RT, FULL>(a, reinterpret_cast<float*>(lds), x.h, t0, r0, n_rows, prefix ? pre : own, lim0, prefix ? 0 : 1, part);
+            __syncthreads();
         }
     }
     if constexpr (DW == 0) {
@@ -1044,6 +1019,14 @@ __global__ __launch_bounds__(kWaves * 64, RT == 1 && D < 256 ? 2 : 1) void k_att
     attention<QT, KT, D, FULL, RT, 0, false>(a, lds);
 }
 
+template <class T, int DN, bool FULL, int RT, int DW, bool WF>
+__global__ __launch_bounds__(kWaves * 64, 2) void k_attn_mixed(Args a) {
+    constexpr int x = narrow_lds<T, T, DN, FULL, RT>(), y = (int)sizeof(WideLds<DW>);
+    __shared__ __attribute__((aligned(16))) char lds[x > y ? x : y];
+    if ((int)blockIdx.x < a.p_items) attention<T, T, DN, FULL, RT, DW, WF>(a, lds);
+    else attention<T, T, DN, FULL, RT, 0, false>(a, lds);
+}
+
 template <class T, int DW, bool WF>
 __global__ __launch_bounds__(kWaves * 64, 2) void k_attn_wide(Args a) {
     __shared__ __attribute__((aligned(16))) char lds[sizeof(WideLds<DW>)];
@@ -1054,6 +1037,8 @@ template <class QT, class KT, int DN, bool FULL, int DW, bool WF>
 void launch_kind(hipStream_t s, const Args& a, Kind kind, unsigned blocks) {
     const dim3 grid(blocks), wg(kWaves * 64);
     if constexpr (DW > 0) {
+        if (kind == kMixed1) { hipLaunchKernelGGL((k_attn_mixed<QT, DN, FULL, 1, DW, WF>), grid, wg, 0, s, a); return; }
+        if (kind == kMixed2) { hipLaunchKernelGGL((k_attn_mixed<QT, DN, FULL, 2, DW, WF>), grid, wg, 0, s, a); return; }
         if (kind == kWide) { hipLaunchKernelGGL((k_attn_wide<QT, DW, WF>), grid, wg, 0, s, a); return; }
     }
     if constexpr (DN < 256) {
