@@ -46,7 +46,6 @@ void split_keys(int64_t want, int64_t round, int64_t keys, int32_t* splits, int3
 struct Plan {
     Kind prefix = pfr::attn::kNarrow1, own = pfr::attn::kNarrow1;
     int64_t prefix_blocks = 0, own_blocks = 0;
-    bool mixed = false;  // the prefix wide, own keys narrow
 };
 
 // Which kernels, and how the work is cut into workgroups.
@@ -56,15 +55,14 @@ Plan plan(int num_cu, bool half,  int64_t max_added, int64_t max_length, int64_t
     const int64_t rows = (int64_t)a.T * a.G, own_rows = max_added * a.G;  // of a key head
     const auto kind = [&](int64_t n) { return half && a.D <= 128 && n > 32 ? kWide : (a.D <= 128 && n > 16 ? kNarrow2 : kNarrow1); };
     const auto tile = [](Kind k) { return k == kWide ? kWideRows : (k == kNarrow2 ? 32 : 16); };
-    const int64_t slots = 2 * num_cu;  // workgroups at a time
-    const int64_t block = half ? kBlock<__bf16> : kBlock<float>, round = kWaves * block, wide_round = 4 * kWideKeys;
+    const int64_t block = half ? kBlock<__bf16> : kBlock<float>, round = kWaves * block, wide_round = EV("X_WR", 4) * kWideKeys;
 
     p.own = kind(own_rows);
-    a.whole = a.B > 0 && p.own == kWide && rows >= 2 * kWideRows * a.B && a.prefix_len + room < INT32_MAX - 4096;
+    a.whole = a.B > 0 && p.own == kWide && rows >= kWideRows * a.B && a.prefix_len + room < INT32_MAX - 4096;
     if (a.whole) {
         a.o_tiles = (int32_t)ceil_div(own_rows, kWideRows);
         const int64_t tiles = a.Hkv * (rows / kWideRows + a.B);
-        split_keys(tiles >= slots ? 1 : ceil_div(slots, tiles), wide_round, a.prefix_len + max_length, &a.o_splits, &a.o_chunk);
+        split_keys(tiles >= num_cu ? 1 : ceil_div(num_cu, tiles), wide_round, a.prefix_len + max_length, &a.o_splits, &a.o_chunk);
         if (a.o_splits == 0) a.o_splits = 1;
     } else {
         p.prefix = kind(rows);
@@ -75,19 +73,14 @@ Plan plan(int num_cu, bool half,  int64_t max_added, int64_t max_length, int64_t
         if (p.prefix != kWide && p.own != kWide) {
             // chunks of one size, four workgroups to a CU if all requests were of max_length
             const int64_t keys = prefix_items * a.prefix_len + own_items * max_length;
-            const int64_t c = ceil_div(ceil_div(keys, 2 * slots), round) * round;
+            const int64_t c = ceil_div(ceil_div(keys, 4 * num_cu), round) * round;
             split_keys(ceil_div(a.prefix_len, c), round, a.prefix_len, &a.p_splits, &a.p_chunk);
             split_keys(ceil_div(max_length, c), round, max_length, &a.o_splits, &a.o_chunk);
         } else {
-            if (EV("X_MIX", 1) && p.own != kWide && own_items > 0) {
-                // the prefix's workgroups, bound by their products, share the CUs with the requests', bound by memory
-                p.mixed = true;
-                split_keys(ceil_div(num_cu * EV("X_P", 100) / 100, prefix_items), wide_round, a.prefix_len, &a.p_splits, &a.p_chunk);
-            } else {
-                split_keys(ceil_div(slots, prefix_items), wide_round, a.prefix_len, &a.p_splits, &a.p_chunk);
-            }
+            split_keys(ceil_div(num_cu, prefix_items), wide_round, a.prefix_len, &a.p_splits, &a.p_chunk);
             if (a.B > 0)
-                split_keys(ceil_div(EV("X_O", 2) * slots, own_items), p.own == kWide ? wide_round : round, max_length, &a.o_splits, &a.o_chunk);
+                split_keys(ceil_div((p.own == kWide ? 1 : 4) * num_cu, own_items), p.own == kWide ? wide_round : round, max_length,
+                           &a.o_splits, &a.o_chunk);
         }
         p.prefix_blocks = (int64_t)a.Hkv * a.p_tiles * a.p_splits;
     }
@@ -104,16 +97,18 @@ __global__ void k_kv_attn_zero(uint32_t* p, int n) {
     if (i < n) p[i] = 0;
 }
 
-// The context's arrival counters, which every launch leaves at zero.
-uint32_t* arrivals(pfr_ctx* ctx, int64_t n) {
-    const size_t had = ctx->scratch[8].bytes, want = (size_t)(n < 16384 ? 16384 : n) * sizeof(uint32_t);
-    auto* p = static_cast<uint32_t*>(ctx->scratch[8].ensure(want));
+// The context's zeros, and n arrival counters, which every launch leaves at zero, behind them.
+constexpr int64_t kZeros = 256;
+char* zeros(pfr_ctx* ctx, int64_t n) {
+    const size_t had = ctx->scratch[8].bytes, want = (size_t)kZeros + (size_t)(n < 16384 ? 16384 : n) * sizeof(uint32_t);
+    void* p = ctx->scratch[8].ensure(want);
     if (ctx->scratch[8].bytes != had) {
         const int words = (int)(ctx->scratch[8].bytes / sizeof(uint32_t));
-        hipLaunchKernelGGL(k_kv_attn_zero, dim3((unsigned)ceil_div(words, 256)), dim3(256), 0, ctx->stream, p, words);
+        hipLaunchKernelGGL(k_kv_attn_zero, dim3((unsigned)ceil_div(words, 256)), dim3(256), 0, ctx->stream,
+                           static_cast<uint32_t*>(p), words);
         PFR_HIP(hipGetLastError());
     }
-    return p;
+    return static_cast<char*>(p);
 }
 
 void enqueue(pfr_ctx* ctx, const pfr_kv* kv, pfr_dtype dtype, const Args& a, Kind kind, int64_t blocks) {
@@ -195,7 +190,9 @@ void attention_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* q, pfr_dtype dtyp
         a.part_o = reinterpret_cast<float*>(ws);
         a.part_ml = reinterpret_cast<float2*>(ws + o);
     }
-    const bool one = p.mixed || p.prefix == p.own;
+    a.zeros = zeros(ctx, a.Hkv * (B + 2));
+    auto* arrived = reinterpret_cast<uint32_t*>(const_cast<char*>(a.zeros) + kZeros);
+    const bool one = p.prefix == p.own;
     const auto by = [](int64_t n) { return pfr::FastDiv((uint32_t)(n > 0 ? n : 1)); };
     a.by_heads = by(a.Hkv);
     a.by_p_tiles = by(a.p_tiles);
@@ -203,11 +200,10 @@ void attention_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* q, pfr_dtype dtyp
     a.by_requests = by(a.B + (a.whole ? 2 : 0));
     // the workgroups that come last join the rows, where few enough requests share the prefix's
     if (a.part_o != nullptr && p.own != pfr::attn::kWide && p.own_blocks > 0 &&
-        (!one || (!p.mixed && B + 2 <= 64 && T * a.G <= 64)))
-        a.arrived = arrivals(ctx, a.Hkv * (B + 2));
+        (!one || (B + 2 <= 64 && T * a.G <= 64)))
+        a.arrived = arrived;
     a.p_items = (int32_t)p.prefix_blocks;
-    const Kind kind = p.mixed ? (p.own == pfr::attn::kNarrow2 ? pfr::attn::kMixed2 : pfr::attn::kMixed1) : p.prefix;
-    enqueue(ctx, kv, dtype, a, kind, p.prefix_blocks + (one ? p.own_blocks : 0));
+    enqueue(ctx, kv, dtype, a, p.prefix, p.prefix_blocks + (one ? p.own_blocks : 0));
     if (!one) {
         a.p_items = 0;
         enqueue(ctx, kv, dtype, a, p.own, p.own_blocks);

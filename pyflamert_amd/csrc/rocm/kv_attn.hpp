@@ -24,7 +24,7 @@ constexpr int kWaves = 4;       // waves of a workgroup
 // product sums over; one keeps a float32 block in registers without spills.
 template <class QT>
 constexpr int kBlock = sizeof(QT) == 2 ? 32 : 16;
-constexpr int kWideRows = 128;  // rows of a workgroup, wide form: 32 a wave
+constexpr int kWideWaves = 8, kWideRows = 32 * kWideWaves;  // waves and rows of a workgroup, wide form
 constexpr int kWideKeys = 64;   // keys of its tile
 constexpr float kSlack = 8.0f;  // how far (log2) scores may pass the number they are weighed against
 
@@ -57,6 +57,7 @@ struct Args {
     // keys; splits are of that whole range.
     FastDiv by_heads, by_p_tiles, by_o_tiles, by_requests;
     int32_t whole, p_items, p_tiles, p_splits, p_chunk, o_tiles, o_splits, o_chunk;
+    const char* zeros;  // 256 of them
     float* part_o;    // [p_splits + o_splits][T * Hq][D], null: rows are whole after one workgroup
     float2* part_ml;  // [p_splits + o_splits][T * Hq]: the score weighed against (log2 units), sum of weights
     // Arrivals at each key head's requests (and at the tokens of none), zero
@@ -65,8 +66,8 @@ struct Args {
 };
 
 // The kernels: narrow (kNarrow1, 2: 16 or 32 rows, waves share the keys) and
-// wide (128 rows, waves share the tile); mixed: the prefix wide, own keys narrow.
-enum Kind { kNarrow1, kNarrow2, kWide, kMixed1, kMixed2 };
+// wide (kWideRows rows, waves share a tile of keys).
+enum Kind { kNarrow1, kNarrow2, kWide };
 
 template <class QT, class KT>
 void launch(hipStream_t s, const Args& a, Kind kind, unsigned blocks);
@@ -267,6 +268,13 @@ __device__ __forceinline__ int here(int x) {
     asm volatile("" : "+v"(x));
     return x;
 }
+
+__device__ __forceinline__ float summed(float x) {  // here, so that its terms are not kept for later
+    asm volatile("" : "+v"(x));
+    return x;
+}
+// The same in all lanes, in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // Whether four 16-bit values hold an infinity or a NaN.
 template <class T>
@@ -485,7 +493,7 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
                 p[rt][u] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[rt][u], a.scale, -ms));
                 sum = sum + p[rt][u];
             }
-            l[rt] = l[rt] + sum;
+            l[rt] = summed(l[rt] + sum);
         }
         if (!poison) {
 #pragma unroll
@@ -587,36 +595,60 @@ constexpr int lds_floats(int cols) {
 
 // ---- wide form: 32 rows a wave, tiles of keys through the LDS ---------------------
 
+constexpr int kStages = 4;     // tiles in the LDS: two arriving, two in use
+constexpr int kWindow = 1024;  // table entries kept there
+
 template <int DP>
 struct WideLds {
     static constexpr int kRow = DP > 64 ? 256 : 128;  // bytes of a key's row
-    alignas(16) char k[2][kWideKeys * kRow];
-    alignas(16) char v[2][kWideKeys * kRow];
-    int64_t off[3][kWideKeys];  // the keys' offsets, -1: absent
-    unsigned long long ok[3];     // which are there
-    uint8_t poison[3][kWideKeys];  // which hold a value that is no number
+    alignas(16) char k[kStages][kWideKeys * kRow];
+    alignas(16) char v[kStages][kWideKeys * kRow];
+    int32_t ids[2][kWindow];
+    uint8_t there[kStages][kWideKeys];
+    uint8_t poison[kStages][kWideKeys];  // which keys hold a value that is no number
 };
 
+// 16 bytes a lane from memory to the LDS, lane i's to byte lds + 16 i.  The
+// compiler does not see these transfers: every read behind them has to wait
+// for them by hand, and no wait that it places counts them.
+__device__ __forceinline__ void transfer(const void* from, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_transfers() {  // until at most N of the wave's are left
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Rows r0 .. of the n_rows that start at token t0 (see narrow) against the keys of
+// pre, which all of them see, and then those of own, of which row r sees the
+// ones below lim0 + r / G.  part < 0: nothing else has a part in these rows.
+//
+// Tiles of 64 keys come to the LDS two tiles ahead, every wave moving its share
+// past the registers; a wave multiplies them with its 32 rows as S^T = K Q^T
+// and O^T = V^T P^T in 32x32x16 products, so that a row's scores, its weights
+// and its column of O^T stay in the lanes n and n + 32.  Waves 4 to 7, which
+// share the SIMDs with waves 0 to 3, take the weights and the second product
+// of a tile one tile later: one wave of a SIMD then has products where the other
+// has exponentials.
 template <class T, int DP, bool FULL>
 __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int t0, int r0, int n_rows, const Seg& pre,
                                      const Seg& own, int lim0, int part) {
     typedef typename Mfma16<T>::V8 V8;
     typedef V8 V8u __attribute__((aligned(2)));
     typedef T V4 __attribute__((ext_vector_type(4)));
-    constexpr int kRow = WideLds<DP>::kRow;
-    constexpr int CPR = DP / 8;   // 16-byte chunks of a key's row
-    constexpr int LPT = DP / 32;  // chunks of K, and of V, a thread moves per tile
+    constexpr int kRow = WideLds<DP>::kRow, kTile = kWideKeys * kRow;
+    constexpr int CP = kRow / 16;          // 16-byte places of a row
+    constexpr int RI = 64 / CP, NI = 8 / RI;  // rows of a transfer, transfers of K (and of V) a wave makes per tile
+    constexpr bool kExact = FULL && DP * 2 == kRow;
     constexpr int QS = DP / 16, DB = DP / 32, KG = QS / 2;
     const int tid = here(threadIdx.x), lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hh = lane >> 5;
     const int np = (pre.hi - pre.lo + kWideKeys - 1) / kWideKeys;
     const int nt = np + (own.hi - own.lo + kWideKeys - 1) / kWideKeys;
 
     // the lane's row
-    const int r = r0 + 32 * w + n;
-    const bool valid = r < n_rows;
-    const int dt = (int)a.group.div((uint32_t)(valid ? r : n_rows - 1));
-    const int hq = h * a.G + (valid ? r : n_rows - 1) - dt * a.G;
-    const int lim = lim0 + dt;
+    const int r = r0 + 32 * w + n, rc = r < n_rows ? r : n_rows - 1;
+    const int dt = (int)a.group.div((uint32_t)rc), lim = lim0 + dt;
     const bool wave_valid = r0 + 32 * w < n_rows;
     // in the own keys: all rows of the workgroup (of the wave) see those below
     const int min_lim = lim0 + (int)a.group.div((uint32_t)r0);
@@ -624,7 +656,7 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
 
     V8 q[QS];
     {
-        const T* row = static_cast<const T*>(a.q) + (int64_t)(t0 + dt) * a.ldq + (int64_t)hq * a.D;
+        const T* row = static_cast<const T*>(a.q) + (int64_t)(t0 + dt) * a.ldq + (int64_t)(h * a.G + rc - dt * a.G) * a.D;
 #pragma unroll
         for (int s = 0; s < QS; ++s) {
             const int d = 16 * s + 8 * hh;
@@ -632,210 +664,234 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
             if (FULL || d < a.D) q[s] = signed_q(V8(*reinterpret_cast<const V8u*>(row + d)), a.sign);
         }
     }
-    f16v o[DB];
+    // q is there before the first transfer: a wait for it later would wait for those too
+#pragma unroll
+    for (int s = 0; s < QS; ++s) {
+        u4 x = __builtin_bit_cast(u4, q[s]);
+        asm volatile("" : "+v"(x));
+        q[s] = __builtin_bit_cast(V8, x);
+    }
+    f16v o[DB], s[2];
 #pragma unroll
     for (int i = 0; i < DB; ++i) o[i] = f16v(0.0f);
     float m = -INFINITY, l = 0.0f;
 
     const T* kp = static_cast<const T*>(a.k) + (int64_t)h * a.head_stride;
     const T* vp = static_cast<const T*>(a.v) + (int64_t)h * a.head_stride;
-    u4 kr[LPT], vr[LPT];
-
     const auto tile_key = [&](int i) { return i < np ? pre.lo + kWideKeys * i : own.lo + kWideKeys * (i - np); };
-    // lane i finds key i of a tile: its table entry, and once that is there its offset
-    const auto find = [&](int i) {
-        const bool p = i < np;
-        return key_place(a.map, tile_key(i) + lane, p ? pre.hi : own.hi);
+    const auto tile_end = [&](int i) { return i < np ? pre.hi : own.hi; };
+
+    // ---- tiles into the LDS.  Row x's chunk c is kept at place c ^ (x & 15)
+    // for K, whose products read a chunk of 16 rows at a time, and c ^ 4 (x &
+    // 3) for V, whose transposed reads take 4 rows x 4 chunks: neither meets
+    // a bank twice (64-element rows: two to 256 bytes, the same by pairs).
+    const unsigned lds_k = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)&lds.k[0][0];
+    const unsigned lds_v = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)&lds.v[0][0];
+    // the window of the table that the tiles being sent for are in
+    const int per_window = (int)(((int64_t)(kWindow - 2) * a.map.page.d) / kWideKeys < (1 << 20)
+                                     ? ((int64_t)(kWindow - 2) * a.map.page.d) / kWideKeys
+                                     : (1 << 20));
+    int win = 0, win_tiles = per_window, win_entry = 0;
+    const auto enter = [&](int i) {  // tile i is the next; whether its window is new and being filled
+        if (i != 0 && i != np && win_tiles < per_window) return false;
+        const int hi = tile_end(i);
+        win ^= 1;
+        win_tiles = 0;
+        win_entry = (int)key_place(a.map, tile_key(i), hi).entry;
+        int left = (int)key_place(a.map, hi - 1, hi).entry - win_entry + 1;
+        left = left < kWindow ? left : kWindow;
+        const int32_t* table = i < np ? pre.table : own.table;
+        for (int x = tid; x < left; x += kWideWaves * 64) lds.ids[win][x] = table[win_entry + x];
+        return true;
     };
-    const auto table_of = [&](int i) { return i < np ? pre.table : own.table; };
-    const auto put = [&](int i, int slot, const KeyPlace& at, int32_t id) {
-        const int64_t off = key_offset(a.map, at, id, tile_key(i) + lane, i < np ? pre.hi : own.hi);
-        lds.off[slot][lane] = off;
-        const unsigned long long ok = __ballot(off >= 0);
-        if (lane == 0) lds.ok[slot] = ok;
-        lds.poison[slot][lane] = 0;
-    };
-    const auto load = [&](int slot) {
+    const auto send = [&](int i) {
+        const int stage = i & (kStages - 1), k0 = tile_key(i), hi = tile_end(i);
+        const int ln = here(lane), place = ln % CP;
 #pragma unroll
-        for (int j = 0; j < LPT; ++j) {
-            const int id = tid + 256 * j, key = id / CPR, c = id % CPR;
-            const int64_t off = lds.off[slot][key];
-            // an absent key: the pool's first row is there to be read, and so is a row's first chunk
-            const int64_t at = (off < 0 ? 0 : off) + (FULL || c * 8 < a.D ? c * 8 : 0);
-            kr[j] = *reinterpret_cast<const u4*>(kp + at);
-            vr[j] = *reinterpret_cast<const u4*>(vp + at);
-        }
-    };
-    // Rows of a tile are kRow bytes apart; chunk c of row x is kept at c ^ (x &
-    // 15) for K, whose products read a chunk of 16 rows at a time, and c ^ 4 (x
-    // & 3) for V, whose transposed reads take 4 rows x 4 chunks: neither
-    // meets a bank twice (64-element rows: two to 256 bytes, the same by pairs).
-    const auto store = [&](int i, int slot, int buf) {
-        const unsigned long long ok = uniform(lds.ok[slot]);
-        const bool partly = i >= np && tile_key(i) + kWideKeys > min_lim;
-        if (ok != ~0ull || partly) {
-#pragma unroll
-            for (int j = 0; j < LPT; ++j) {
-                const int key = (tid + 256 * j) / CPR;
-                if (!((ok >> key) & 1)) vr[j] = u4(0);
-                if (partly) {
-                    // four values with one that is no number: kept from the rows that do not see them, see below
-                    const bool x = nonfinite<T>(vr[j][0], vr[j][1]), y = nonfinite<T>(vr[j][2], vr[j][3]);
-                    if (x) vr[j][0] = vr[j][1] = 0;
-                    if (y) vr[j][2] = vr[j][3] = 0;
-                    if (x || y) lds.poison[slot][key] = 1;
-                }
+        for (int b = 0; b < NI; ++b) {
+            const int row = 8 * w + RI * b + ln / CP, key = k0 + row;
+            const KeyPlace at = key_place(a.map, key, hi);
+            const int64_t off = key_offset(a.map, at, lds.ids[win][at.entry - win_entry], key, hi);
+            const int fk = kRow == 256 ? row & 15 : (row >> 1) & 7, fv = kRow == 256 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
+            const int ck = place ^ fk, cv = place ^ fv;
+            // absent keys, and chunks past D, are zeros
+            const char* zero = a.zeros + place * 16;
+            const void* gk = off >= 0 && (kExact || ck * 8 < a.D) ? reinterpret_cast<const char*>(kp + off + ck * 8) : zero;
+            const void* gv = off >= 0 && (kExact || cv * 8 < a.D) ? reinterpret_cast<const char*>(vp + off + cv * 8) : zero;
+            const unsigned to = (unsigned)(stage * kTile + (8 * w + RI * b) * kRow);
+            transfer(gk, lds_k + to);
+            transfer(gv, lds_v + to);
+            if (place == 0) {
+                lds.there[stage][row] = off >= 0;
+                lds.poison[stage][row] = 0;
             }
         }
+        ++win_tiles;
+    };
+    // Of a tile that only some rows see whole: four values with one that is no number
+    // are cleared, for 0 times it is no number either; see below.
+    const auto patch = [&](int i) {
+        if (i < np || tile_key(i) + kWideKeys <= min_lim) return;
+        const int stage = i & (kStages - 1), ln = here(lane), place = ln % CP;
 #pragma unroll
-        for (int j = 0; j < LPT; ++j) {
-            const int id = tid + 256 * j, key = id / CPR, c = id % CPR;
-            const int fk = kRow == 256 ? key & 15 : (key >> 1) & 7, fv = kRow == 256 ? (key & 3) << 2 : ((key >> 1) & 1) << 2;
-            if (!FULL && c * 8 >= a.D) kr[j] = vr[j] = u4(0);
-            *reinterpret_cast<u4*>(lds.k[buf] + key * kRow + ((c ^ fk) << 4)) = kr[j];
-            *reinterpret_cast<u4*>(lds.v[buf] + key * kRow + ((c ^ fv) << 4)) = vr[j];
+        for (int b = 0; b < NI; ++b) {
+            const int row = 8 * w + RI * b + ln / CP;
+            u4* at = reinterpret_cast<u4*>(lds.v[stage] + row * kRow + place * 16);
+            u4 x = *at;
+            const bool lo = nonfinite<T>(x[0], x[1]), hi = nonfinite<T>(x[2], x[3]);
+            if (lo || hi) {
+                if (lo) x[0] = x[1] = 0;
+                if (hi) x[2] = x[3] = 0;
+                *at = x;
+                lds.poison[stage][row] = 1;
+            }
         }
     };
 
-    if (nt > 0) {
-        if (w < 2 && w < nt) {
-            const KeyPlace at = find(w);
-            put(w, w, at, table_of(w)[at.entry]);
-        }
-        __syncthreads();
-        load(0);
-        store(0, 0, 0);
-        __syncthreads();
-    }
-    const int kat = n * kRow + (((kRow == 256 ? n & 15 : (n >> 1) & 7) ^ hh) << 4);
-    // transposed read: lane 4 e + x of 16 holds row e's columns 4 x .., and lane
-    // i gets column i of the four rows
-    const int vrow = 4 * hh + ((lane & 15) >> 2);
-    const int vsw = kRow == 256 ? vrow & 3 : (vrow >> 1) & 1;
-    const int vat = vrow * kRow + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) << 4) + (lane & 1) * 8;
-
-    int slot = 0;
-    for (int i = 0; i < nt; ++i) {
-        const int slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot1 == 2 ? 0 : slot1 + 1, buf = i & 1;
-        // The table first, so that what needs it does not wait for the rows; and no
-        // branch around a load: with one, waits for older loads would wait for it too.
-        const int i2 = i + 2 < nt ? i + 2 : nt - 1;
-        const KeyPlace at2 = find(i2);
-        const int32_t id2 = table_of(i2)[at2.entry];
-        load(i + 1 < nt ? slot1 : slot);
-        const int k0 = tile_key(i);
-        const bool mine = i >= np;
-        if (wave_valid && (!mine || k0 < wave_max)) {
-            const char* kb = lds.k[buf];
-            const char* vb = lds.v[buf];
-            f16v s[2];
-            // Four groups of fragments of K, then of V, each read while the one before is multiplied.
-            V8 kf[2][KG];
-            const auto read_k = [&](int g) {
+    // ---- the products
+    const auto active = [&](int i) { return wave_valid && (i < np || tile_key(i) < wave_max); };
+    const auto scores = [&](int i) {
+        const char* kb = lds.k[i & (kStages - 1)];
+        const int kn = here(n), kat = kn * kRow + (((kRow == 256 ? kn & 15 : (kn >> 1) & 7) ^ hh) << 4);
+        // Four groups of fragments, each read while the one before is multiplied.
+        V8 kf[2][KG];
+        const auto read_k = [&](int g) {
 #pragma unroll
-                for (int j = 0; j < KG; ++j)
-                    kf[g & 1][j] = *reinterpret_cast<const V8*>(kb + (g >> 1) * 32 * kRow + (kat ^ ((j + (g & 1) * KG) << 5)));
-            };
-            read_k(0);
+            for (int j = 0; j < KG; ++j)
+                kf[g & 1][j] = *reinterpret_cast<const V8*>(kb + (g >> 1) * 32 * kRow + (kat ^ ((j + (g & 1) * KG) << 5)));
+        };
+        read_k(0);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                __builtin_amdgcn_sched_barrier(0);
-                if (g < 3) read_k(g + 1);
-#pragma unroll
-                for (int j = 0; j < KG; ++j)
-                    s[g >> 1] = Mfma16<T>::dot32(kf[g & 1][j], q[j + (g & 1) * KG], (g & 1) == 0 && j == 0 ? f16v(0.0f) : s[g >> 1]);
-            }
+        for (int g = 0; g < 4; ++g) {
             __builtin_amdgcn_sched_barrier(0);
-            const unsigned long long ok = uniform(lds.ok[slot]);
-            if (ok != ~0ull || (mine && k0 + kWideKeys > wave_min)) {
-                const int see = mine ? lim - k0 : kWideKeys;
-                unsigned long long there = ok & (see >= kWideKeys ? ~0ull : (see <= 0 ? 0ull : (1ull << see) - 1));
-                there >>= 4 * hh;
+            if (g < 3) read_k(g + 1);
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+            for (int j = 0; j < KG; ++j)
+                s[g >> 1] = Mfma16<T>::dot32(kf[g & 1][j], q[j + (g & 1) * KG], (g & 1) == 0 && j == 0 ? f16v(0.0f) : s[g >> 1]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const auto weigh = [&](int i) {
+        const int stage = i & (kStages - 1), k0 = tile_key(i);
+        const bool mine = i >= np;
+        const char* vb = lds.v[stage];
+        // transposed read: lane 4 e + x of 16 holds row e's columns 4 x .., and lane
+        // i gets column i of the four rows
+        const int ln = here(lane), vrow = 4 * (ln >> 5) + ((ln & 15) >> 2), vsw = kRow == 256 ? vrow & 3 : (vrow >> 1) & 1;
+        const int vat = vrow * kRow + ((2 * ((ln >> 4) & 1) + ((ln & 3) >> 1)) << 4) + (ln & 1) * 8;
+        V8 vf[2][DB];
+        const auto read_v = [&](int g) {
 #pragma unroll
-                    for (int x = 0; x < 16; ++x)
-                        s[b][x] = (unsigned)(there >> 32 * b) & (1u << (8 * (x >> 2) + (x & 3))) ? s[b][x] : -INFINITY;
+            for (int d = 0; d < DB; ++d) {
+                const char* at = vb + 16 * g * kRow + vat + ((d ^ vsw) << 6);
+                const s4 lo = read_tr(at), hi = read_tr(at + 8 * kRow);
+                vf[g & 1][d] = __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
             }
-            float mx = s[0][0];
-#pragma unroll
-            for (int x = 1; x < 16; ++x) mx = fmaxf(mx, s[0][x]);
-#pragma unroll
-            for (int x = 0; x < 16; ++x) mx = fmaxf(mx, s[1][x]);
-            mx = fmaxf(mx, half_swap(mx));
-            const float mn = fmaxf(m, mx * a.scale);
-            // m only has to be near the largest score: weights up to 2^kSlack fit every type
-            if (__any(mn > m + kSlack)) {
-                const float alpha = __builtin_amdgcn_exp2f(m - finite_max(mn));
-                l *= alpha;
-#pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] *= alpha;
-                m = mn;
-            }
-            const float ms = finite_max(m);
-            V8 p[2][2];
-            float sum = 0.0f;
+        };
+        const unsigned long long ok = __ballot(lds.there[stage][lane] != 0);
+        if (ok != ~0ull || (mine && k0 + kWideKeys > wave_min)) {
+            const int see = mine ? lim - k0 : kWideKeys;
+            unsigned long long there = ok & (see >= kWideKeys ? ~0ull : (see <= 0 ? 0ull : (1ull << see) - 1));
+            there >>= 4 * hh;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][x], a.scale, -ms));
-                    sum = sum + e;
-                    p[b][x >> 3][x & 7] = (T)e;
-                }
-            l = l + sum;
-            V8 vf[2][DB];
-            const auto read_v = [&](int g) {
+                for (int x = 0; x < 16; ++x)
+                    s[b][x] = (unsigned)(there >> 32 * b) & (1u << (8 * (x >> 2) + (x & 3))) ? s[b][x] : -INFINITY;
+        }
+        float mx = s[0][0];
 #pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    const char* at = vb + 16 * g * kRow + vat + ((d ^ vsw) << 6);
-                    const s4 lo = read_tr(at), hi = read_tr(at + 8 * kRow);
-                    vf[g & 1][d] = __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-                }
-            };
-            read_v(0);
+        for (int x = 1; x < 16; ++x) mx = fmaxf(mx, s[0][x]);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                __builtin_amdgcn_sched_barrier(0);
-                if (g < 3) read_v(g + 1);
+        for (int x = 0; x < 16; ++x) mx = fmaxf(mx, s[1][x]);
+        mx = fmaxf(mx, half_swap(mx));
+        const float mn = fmaxf(m, mx * a.scale);
+        // m only has to be near the largest score: weights up to 2^kSlack fit every type
+        if (__any(mn > m + kSlack)) {
+            const float alpha = __builtin_amdgcn_exp2f(m - finite_max(mn));
+            l *= alpha;
 #pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] = Mfma16<T>::dot32(vf[g & 1][d], p[g >> 1][g & 1], o[d]);
+            for (int d = 0; d < DB; ++d) o[d] *= alpha;
+            m = mn;
+        }
+        const float ms = finite_max(m);
+        V8 p[2][2];
+        float sum = 0.0f;
+        read_v(0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][x], a.scale, -ms));
+                sum = sum + e;
+                p[b][x >> 3][x & 7] = (T)e;
             }
+        l = summed(l + sum);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
             __builtin_amdgcn_sched_barrier(0);
-            unsigned long long poison = mine && k0 + kWideKeys > min_lim ? __ballot(lds.poison[slot][lane] != 0) : 0;
-            // A key that only some rows see must not reach the others, and 0 times
-            // an infinity or a NaN would: such values are added row by row.
-            for (; poison; poison &= poison - 1) {
-                const int kk = __builtin_ctzll(poison), at = ((kk >> 3) & 3) * 4 + (kk & 3);
-                float pk = 0.0f;
+            if (g < 3) read_v(g + 1);
 #pragma unroll
-                for (int x = 0; x < 16; ++x) pk = x == at ? (float)(kk < 32 ? p[0][x >> 3][x & 7] : p[1][x >> 3][x & 7]) : pk;
-                pk = __shfl(pk, (kk & 4) * 8 + n);
-                const T* row = vp + lds.off[slot][kk];
-                if (k0 + kk < lim) {
+            for (int d = 0; d < DB; ++d) o[d] = Mfma16<T>::dot32(vf[g & 1][d], p[g >> 1][g & 1], o[d]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // A key that only some rows see must not reach the others: what patch() cleared is
+        // added to the rows that do.
+        unsigned long long poison = mine && k0 + kWideKeys > min_lim ? __ballot(lds.poison[stage][lane] != 0) : 0;
+        for (; poison; poison &= poison - 1) {
+            const int kk = __builtin_ctzll(poison), at = ((kk >> 3) & 3) * 4 + (kk & 3), key = k0 + kk;
+            float pk = 0.0f;
 #pragma unroll
-                    for (int d = 0; d < DB; ++d)
+            for (int x = 0; x < 16; ++x) pk = x == at ? (float)(kk < 32 ? p[0][x >> 3][x & 7] : p[1][x >> 3][x & 7]) : pk;
+            pk = __shfl(pk, (kk & 4) * 8 + n);
+            const KeyPlace place = key_place(a.map, key, own.hi);
+            const T* row = vp + key_offset(a.map, place, own.table[place.entry], key, own.hi);  // there, or it would be zeros
+            if (key < lim) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int c = 32 * d + 8 * j + 4 * hh;
-                            if (FULL || c < a.D) {
-                                const V4 x = *reinterpret_cast<const V4*>(row + c);
-                                const u2 y = __builtin_bit_cast(u2, x);
-                                if (nonfinite<T>(y[0], y[1])) {
+                for (int d = 0; d < DB; ++d)
 #pragma unroll
-                                    for (int e = 0; e < 4; ++e) o[d][4 * j + e] += pk * (float)x[e];
-                                }
+                    for (int j = 0; j < 4; ++j) {
+                        const int c = 32 * d + 8 * j + 4 * hh;
+                        if (FULL || c < a.D) {
+                            const V4 x = *reinterpret_cast<const V4*>(row + c);
+                            const u2 y = __builtin_bit_cast(u2, x);
+                            if (nonfinite<T>(y[0], y[1])) {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[d][4 * j + e] += pk * (float)x[e];
                             }
-                            __builtin_amdgcn_sched_barrier(0);  // not all of them in registers at once
                         }
-                }
+                        __builtin_amdgcn_sched_barrier(0);  // not all of them in registers at once
+                    }
             }
         }
-        if (i + 2 < nt && w == (i & 3)) put(i2, slot2, at2, id2);
-        if (i + 1 < nt) store(i + 1, slot1, buf ^ 1);
-        __syncthreads();
-        slot = slot1;
+    };
+
+    const bool late = w >= kWideWaves / 2;
+    for (int i = 0; i < 2 && i < nt; ++i) {
+        if (enter(i)) lds_barrier();
+        send(i);
     }
+    // the same barriers either way
+    const auto tiles = [&](auto second) {
+        constexpr bool kLate = decltype(second)::value;
+        for (int i = 0; i <= nt; ++i) {
+            if (i + 1 < nt) wait_transfers<2 * NI>();  // all but the next tile's
+            else wait_transfers<0>();
+            if (i < nt) patch(i);
+            if (i + 2 < nt) enter(i + 2);
+            lds_barrier();  // tile i is there for all, tile i - 2 done with
+            if (i + 2 < nt) send(i + 2);
+            if (kLate && i > 0 && active(i - 1)) weigh(i - 1);
+            if (i < nt && active(i)) {
+                scores(i);
+                if (!kLate) weigh(i);
+            }
+        }
+    };
+    if (late) tiles(std::true_type());
+    else tiles(std::false_type());
+    lds_barrier();
 
     l = l + half_swap(l);
     const int er = r0 + 32 * w + here(n), eh = here(hh);
@@ -909,7 +965,7 @@ __device__ __forceinline__ Item item_of(const Args& a) {
 
 // No keys for rows [r0, r1) of a part: the join skips what has no weight.
 __device__ __forceinline__ void no_keys(const Args& a, int h, int t0, int r0, int r1, int part) {
-    for (int r = r0 + (int)threadIdx.x; r < r1; r += kWaves * 64) {
+    for (int r = r0 + (int)threadIdx.x; r < r1; r += (int)blockDim.x) {
         const int dt = (int)a.group.div((uint32_t)r);
         put_pair(a.part_ml + (int64_t)part * a.T * a.Hq + (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G), -INFINITY, 0.0f);
     }
@@ -973,6 +1029,9 @@ __device__ __forceinline__ void attention(const Args& a, char* lds) {
             room = (int64_t)a.table_w * a.map.page.d;
             table = a.table + (int64_t)x.b * a.table_ld;
         }
+        t0 = uniform(t0);
+        t1 = uniform(t1);
+        lim0 = uniform(lim0);
         if (!a.whole) P = 0;
         part = a.part_o == nullptr ? -1 : a.p_splits + x.split;
         tiles_apart = a.o_tiles;
@@ -985,6 +1044,8 @@ __device__ __forceinline__ void attention(const Args& a, char* lds) {
         const int end = prefix ? 0 : keys_end(lim0, (int)a.group.div((uint32_t)(r1 - 1)), room);
         int lo, hi;  // of the prefix and the own keys behind it
         split_span(x.split, splits, chunk, P + end, &lo, &hi);
+        lo = uniform(lo);
+        hi = uniform(hi);
         if (part >= 0 && lo == hi) {
             no_keys(a, x.h, t0, r0, r1, part);
             continue;
@@ -1019,16 +1080,8 @@ __global__ __launch_bounds__(kWaves * 64, RT == 1 && D < 256 ? 2 : 1) void k_att
     attention<QT, KT, D, FULL, RT, 0, false>(a, lds);
 }
 
-template <class T, int DN, bool FULL, int RT, int DW, bool WF>
-__global__ __launch_bounds__(kWaves * 64, 2) void k_attn_mixed(Args a) {
-    constexpr int x = narrow_lds<T, T, DN, FULL, RT>(), y = (int)sizeof(WideLds<DW>);
-    __shared__ __attribute__((aligned(16))) char lds[x > y ? x : y];
-    if ((int)blockIdx.x < a.p_items) attention<T, T, DN, FULL, RT, DW, WF>(a, lds);
-    else attention<T, T, DN, FULL, RT, 0, false>(a, lds);
-}
-
 template <class T, int DW, bool WF>
-__global__ __launch_bounds__(kWaves * 64, 2) void k_attn_wide(Args a) {
+__global__ __launch_bounds__(kWideWaves * 64, 2) void k_attn_wide(Args a) {
     __shared__ __attribute__((aligned(16))) char lds[sizeof(WideLds<DW>)];
     attention<T, T, 64, false, 1, DW, WF>(a, lds);
 }
@@ -1037,9 +1090,7 @@ template <class QT, class KT, int DN, bool FULL, int DW, bool WF>
 void launch_kind(hipStream_t s, const Args& a, Kind kind, unsigned blocks) {
     const dim3 grid(blocks), wg(kWaves * 64);
     if constexpr (DW > 0) {
-        if (kind == kMixed1) { hipLaunchKernelGGL((k_attn_mixed<QT, DN, FULL, 1, DW, WF>), grid, wg, 0, s, a); return; }
-        if (kind == kMixed2) { hipLaunchKernelGGL((k_attn_mixed<QT, DN, FULL, 2, DW, WF>), grid, wg, 0, s, a); return; }
-        if (kind == kWide) { hipLaunchKernelGGL((k_attn_wide<QT, DW, WF>), grid, wg, 0, s, a); return; }
+        if (kind == kWide) { hipLaunchKernelGGL((k_attn_wide<QT, DW, WF>), grid, dim3(kWideWaves * 64), 0, s, a); return; }
     }
     if constexpr (DN < 256) {
         if (kind == kNarrow2) { hipLaunchKernelGGL((k_attn_narrow<QT, KT, DN, FULL, 2>), grid, wg, 0, s, a); return; }
