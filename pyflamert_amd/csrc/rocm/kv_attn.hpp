@@ -596,6 +596,7 @@ constexpr int lds_floats(int cols) {
 // ---- wide form: 32 rows a wave, tiles of keys through the LDS ---------------------
 
 constexpr int kStages = 4;     // tiles in the LDS: two arriving, two in use
+constexpr int kFound = 8;      // tiles whose keys are found: from three ahead to one behind
 constexpr int kWindow = 1024;  // table entries kept there
 
 template <int DP>
@@ -604,8 +605,9 @@ struct WideLds {
     alignas(16) char k[kStages][kWideKeys * kRow];
     alignas(16) char v[kStages][kWideKeys * kRow];
     int32_t ids[2][kWindow];
-    uint8_t there[kStages][kWideKeys];
-    uint8_t poison[kStages][kWideKeys];  // which keys hold a value that is no number
+    int64_t off[kFound][kWideKeys];  // the keys' offsets, -1: absent
+    unsigned long long there[kFound];   // which are there
+    uint8_t poison[kFound][kWideKeys];  // which keys hold a value that is no number
 };
 
 // 16 bytes a lane from memory to the LDS, lane i's to byte lds + 16 i.  The
@@ -641,7 +643,7 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
     constexpr int CP = kRow / 16;          // 16-byte places of a row
     constexpr int RI = 64 / CP, NI = 8 / RI;  // rows of a transfer, transfers of K (and of V) a wave makes per tile
     constexpr bool kExact = FULL && DP * 2 == kRow;
-    constexpr int QS = DP / 16, DB = DP / 32, KG = QS / 2;
+    constexpr int QS = DP / 16, DB = DP / 32;
     const int tid = here(threadIdx.x), lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 31, hh = lane >> 5;
     const int np = (pre.hi - pre.lo + kWideKeys - 1) / kWideKeys;
     const int nt = np + (own.hi - own.lo + kWideKeys - 1) / kWideKeys;
@@ -692,11 +694,14 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
                                      ? ((int64_t)(kWindow - 2) * a.map.page.d) / kWideKeys
                                      : (1 << 20));
     int win = 0, win_tiles = per_window, win_entry = 0;
-    const auto enter = [&](int i) {  // tile i is the next; whether its window is new and being filled
-        if (i != 0 && i != np && win_tiles < per_window) return false;
+    const auto enter = [&](int i) {  // tile i is the next to be found; whether its window is new and being filled
+        if (i != 0 && i != np && win_tiles < per_window) {
+            ++win_tiles;
+            return false;
+        }
         const int hi = tile_end(i);
         win ^= 1;
-        win_tiles = 0;
+        win_tiles = 1;
         win_entry = (int)key_place(a.map, tile_key(i), hi).entry;
         int left = (int)key_place(a.map, hi - 1, hi).entry - win_entry + 1;
         left = left < kWindow ? left : kWindow;
@@ -704,29 +709,33 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
         for (int x = tid; x < left; x += kWideWaves * 64) lds.ids[win][x] = table[win_entry + x];
         return true;
     };
+    // a wave finds the keys of tile i, one a lane
+    const auto find = [&](int i) {
+        const int slot = i & (kFound - 1), key = tile_key(i) + lane, hi = tile_end(i);
+        const KeyPlace at = key_place(a.map, key, hi);
+        const int64_t off = key_offset(a.map, at, lds.ids[win][at.entry - win_entry], key, hi);
+        lds.off[slot][lane] = off;
+        lds.poison[slot][lane] = 0;
+        const unsigned long long there = __ballot(off >= 0);
+        if (lane == 0) lds.there[slot] = there;
+    };
     const auto send = [&](int i) {
-        const int stage = i & (kStages - 1), k0 = tile_key(i), hi = tile_end(i);
+        const int stage = i & (kStages - 1);
         const int ln = here(lane), place = ln % CP;
 #pragma unroll
         for (int b = 0; b < NI; ++b) {
-            const int row = 8 * w + RI * b + ln / CP, key = k0 + row;
-            const KeyPlace at = key_place(a.map, key, hi);
-            const int64_t off = key_offset(a.map, at, lds.ids[win][at.entry - win_entry], key, hi);
+            const int row = 8 * w + RI * b + ln / CP;
+            const int64_t off = lds.off[i & (kFound - 1)][row];
             const int fk = kRow == 256 ? row & 15 : (row >> 1) & 7, fv = kRow == 256 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
             const int ck = place ^ fk, cv = place ^ fv;
             // absent keys, and chunks past D, are zeros
             const char* zero = a.zeros + place * 16;
-            const void* gk = off >= 0 && (kExact || ck * 8 < a.D) ? reinterpret_cast<const char*>(kp + off + ck * 8) : zero;
-            const void* gv = off >= 0 && (kExact || cv * 8 < a.D) ? reinterpret_cast<const char*>(vp + off + cv * 8) : zero;
+            const void* gk = off >= 0 && (kExact || ck * 8 < a.D) ? reinterpret_cast<const char*>(kp + ck * 8 + off) : zero;
+            const void* gv = off >= 0 && (kExact || cv * 8 < a.D) ? reinterpret_cast<const char*>(vp + cv * 8 + off) : zero;
             const unsigned to = (unsigned)(stage * kTile + (8 * w + RI * b) * kRow);
             transfer(gk, lds_k + to);
             transfer(gv, lds_v + to);
-            if (place == 0) {
-                lds.there[stage][row] = off >= 0;
-                lds.poison[stage][row] = 0;
-            }
         }
-        ++win_tiles;
     };
     // Of a tile that only some rows see whole: four values with one that is no number
     // are cleared, for 0 times it is no number either; see below.
@@ -743,7 +752,7 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
                 if (lo) x[0] = x[1] = 0;
                 if (hi) x[2] = x[3] = 0;
                 *at = x;
-                lds.poison[stage][row] = 1;
+                lds.poison[i & (kFound - 1)][row] = 1;
             }
         }
     };
@@ -753,21 +762,22 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
     const auto scores = [&](int i) {
         const char* kb = lds.k[i & (kStages - 1)];
         const int kn = here(n), kat = kn * kRow + (((kRow == 256 ? kn & 15 : (kn >> 1) & 7) ^ hh) << 4);
-        // Four groups of fragments, each read while the one before is multiplied.
-        V8 kf[2][KG];
+        // Groups of four fragments, of both halves of the tile, each read while the
+        // one before is multiplied.
+        V8 kf[2][4];
         const auto read_k = [&](int g) {
 #pragma unroll
-            for (int j = 0; j < KG; ++j)
-                kf[g & 1][j] = *reinterpret_cast<const V8*>(kb + (g >> 1) * 32 * kRow + (kat ^ ((j + (g & 1) * KG) << 5)));
+            for (int j = 0; j < 4; ++j)
+                kf[g & 1][j] = *reinterpret_cast<const V8*>(kb + (j & 1) * 32 * kRow + (kat ^ ((2 * g + (j >> 1)) << 5)));
         };
         read_k(0);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
+        for (int g = 0; g < QS / 2; ++g) {
             __builtin_amdgcn_sched_barrier(0);
-            if (g < 3) read_k(g + 1);
+            if (g + 1 < QS / 2) read_k(g + 1);
 #pragma unroll
-            for (int j = 0; j < KG; ++j)
-                s[g >> 1] = Mfma16<T>::dot32(kf[g & 1][j], q[j + (g & 1) * KG], (g & 1) == 0 && j == 0 ? f16v(0.0f) : s[g >> 1]);
+            for (int j = 0; j < 4; ++j)
+                s[j & 1] = Mfma16<T>::dot32(kf[g & 1][j], q[2 * g + (j >> 1)], g == 0 && j < 2 ? f16v(0.0f) : s[j & 1]);
         }
         __builtin_amdgcn_sched_barrier(0);
     };
@@ -788,7 +798,7 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
                 vf[g & 1][d] = __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
             }
         };
-        const unsigned long long ok = __ballot(lds.there[stage][lane] != 0);
+        const unsigned long long ok = uniform(lds.there[i & (kFound - 1)]);
         if (ok != ~0ull || (mine && k0 + kWideKeys > wave_min)) {
             const int see = mine ? lim - k0 : kWideKeys;
             unsigned long long there = ok & (see >= kWideKeys ? ~0ull : (see <= 0 ? 0ull : (1ull << see) - 1));
@@ -838,7 +848,7 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
         __builtin_amdgcn_sched_barrier(0);
         // A key that only some rows see must not reach the others: what patch() cleared is
         // added to the rows that do.
-        unsigned long long poison = mine && k0 + kWideKeys > min_lim ? __ballot(lds.poison[stage][lane] != 0) : 0;
+        unsigned long long poison = mine && k0 + kWideKeys > min_lim ? __ballot(lds.poison[i & (kFound - 1)][lane] != 0) : 0;
         for (; poison; poison &= poison - 1) {
             const int kk = __builtin_ctzll(poison), at = ((kk >> 3) & 3) * 4 + (kk & 3), key = k0 + kk;
             float pk = 0.0f;
@@ -868,10 +878,12 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
     };
 
     const bool late = w >= kWideWaves / 2;
-    for (int i = 0; i < 2 && i < nt; ++i) {
+    for (int i = 0; i < 3 && i < nt; ++i) {
         if (enter(i)) lds_barrier();
-        send(i);
+        if (w == i) find(i);
     }
+    lds_barrier();
+    for (int i = 0; i < 2 && i < nt; ++i) send(i);
     // the same barriers either way
     const auto tiles = [&](auto second) {
         constexpr bool kLate = decltype(second)::value;
@@ -879,9 +891,10 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
             if (i + 1 < nt) wait_transfers<2 * NI>();  // all but the next tile's
             else wait_transfers<0>();
             if (i < nt) patch(i);
-            if (i + 2 < nt) enter(i + 2);
+            if (i + 3 < nt) enter(i + 3);
             lds_barrier();  // tile i is there for all, tile i - 2 done with
             if (i + 2 < nt) send(i + 2);
+            if (i + 3 < nt && w == (i & (kWideWaves - 1))) find(i + 3);
             if (kLate && i > 0 && active(i - 1)) weigh(i - 1);
             if (i < nt && active(i)) {
                 scores(i);
