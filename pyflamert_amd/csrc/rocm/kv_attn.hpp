@@ -370,8 +370,8 @@ __device__ __forceinline__ void join_row(const Args& a, int64_t R, int t, int pa
 
 // Four 16-bit elements a lane of a tile in the LDS, transposed among 16 lanes:
 // lane i gets element i % 4 of what lanes i / 4, i / 4 + 4, .. + 12 address.
-__device__ __forceinline__ s4 read_tr(const char* p) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
+__device__ __forceinline__ s4 read_tr(unsigned lds) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)lds);
 }
 
 // One workgroup's rows against keys [lo, hi) of one table.  Rows r0 .. of the
@@ -629,10 +629,8 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // Tiles of 64 keys come to the LDS two tiles ahead, every wave moving its share
 // past the registers; a wave multiplies them with its 32 rows as S^T = K Q^T
 // and O^T = V^T P^T in 32x32x16 products, so that a row's scores, its weights
-// and its column of O^T stay in the lanes n and n + 32.  Waves 4 to 7, which
-// share the SIMDs with waves 0 to 3, take the weights and the second product
-// of a tile one tile later: one wave of a SIMD then has products where the other
-// has exponentials.
+// and its column of O^T stay in the lanes n and n + 32.  The second product of
+// a tile runs beside the exponentials of the next.
 template <class T, int DP, bool FULL>
 __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int t0, int r0, int n_rows, const Seg& pre,
                                      const Seg& own, int lim0, int part) {
@@ -654,7 +652,7 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
     const bool wave_valid = r0 + 32 * w < n_rows;
     // in the own keys: all rows of the workgroup (of the wave) see those below
     const int min_lim = lim0 + (int)a.group.div((uint32_t)r0);
-    const int wave_min = __builtin_amdgcn_readfirstlane(lim), wave_max = __builtin_amdgcn_readlane(lim, 31);
+    const int wave_min = __builtin_amdgcn_readfirstlane(lim);
 
     V8 q[QS];
     {
@@ -719,32 +717,40 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
         const unsigned long long there = __ballot(off >= 0);
         if (lane == 0) lds.there[slot] = there;
     };
+    // what the lane moves: of row 8 w + RI b + lane / CP the chunks that are kept at its place
+    const int place = lane % CP;
+    const T *from_k[NI], *from_v[NI];
+    bool is_k[NI], is_v[NI];  // chunks before D
+#pragma unroll
+    for (int b = 0; b < NI; ++b) {
+        const int row = 8 * w + RI * b + lane / CP;
+        const int ck = place ^ (kRow == 256 ? row & 15 : (row >> 1) & 7);
+        const int cv = place ^ (kRow == 256 ? (row & 3) << 2 : ((row >> 1) & 1) << 2);
+        from_k[b] = kp + ck * 8;
+        from_v[b] = vp + cv * 8;
+        is_k[b] = kExact || ck * 8 < a.D;
+        is_v[b] = kExact || cv * 8 < a.D;
+    }
     const auto send = [&](int i) {
-        const int stage = i & (kStages - 1);
-        const int ln = here(lane), place = ln % CP;
+        const int64_t* found = lds.off[i & (kFound - 1)] + 8 * w + lane / CP;
+        const unsigned to = (unsigned)((i & (kStages - 1)) * kTile + 8 * w * kRow);
 #pragma unroll
         for (int b = 0; b < NI; ++b) {
-            const int row = 8 * w + RI * b + ln / CP;
-            const int64_t off = lds.off[i & (kFound - 1)][row];
-            const int fk = kRow == 256 ? row & 15 : (row >> 1) & 7, fv = kRow == 256 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
-            const int ck = place ^ fk, cv = place ^ fv;
+            const int64_t off = found[RI * b];
+            const bool there = off >= 0;
             // absent keys, and chunks past D, are zeros
-            const char* zero = a.zeros + place * 16;
-            const void* gk = off >= 0 && (kExact || ck * 8 < a.D) ? reinterpret_cast<const char*>(kp + ck * 8 + off) : zero;
-            const void* gv = off >= 0 && (kExact || cv * 8 < a.D) ? reinterpret_cast<const char*>(vp + cv * 8 + off) : zero;
-            const unsigned to = (unsigned)(stage * kTile + (8 * w + RI * b) * kRow);
-            transfer(gk, lds_k + to);
-            transfer(gv, lds_v + to);
+            transfer(there && is_k[b] ? static_cast<const void*>(from_k[b] + off) : a.zeros, lds_k + to + RI * b * kRow);
+            transfer(there && is_v[b] ? static_cast<const void*>(from_v[b] + off) : a.zeros, lds_v + to + RI * b * kRow);
         }
     };
     // Of a tile that only some rows see whole: four values with one that is no number
     // are cleared, for 0 times it is no number either; see below.
     const auto patch = [&](int i) {
         if (i < np || tile_key(i) + kWideKeys <= min_lim) return;
-        const int stage = i & (kStages - 1), ln = here(lane), place = ln % CP;
+        const int stage = i & (kStages - 1);
 #pragma unroll
         for (int b = 0; b < NI; ++b) {
-            const int row = 8 * w + RI * b + ln / CP;
+            const int row = 8 * w + RI * b + lane / CP;
             u4* at = reinterpret_cast<u4*>(lds.v[stage] + row * kRow + place * 16);
             u4 x = *at;
             const bool lo = nonfinite<T>(x[0], x[1]), hi = nonfinite<T>(x[2], x[3]);
@@ -758,17 +764,16 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
     };
 
     // ---- the products
-    const auto active = [&](int i) { return wave_valid && (i < np || tile_key(i) < wave_max); };
+    const unsigned k_at = lds_k + n * kRow + (((kRow == 256 ? n & 15 : (n >> 1) & 7) ^ hh) << 4);
     const auto scores = [&](int i) {
-        const char* kb = lds.k[i & (kStages - 1)];
-        const int kn = here(n), kat = kn * kRow + (((kRow == 256 ? kn & 15 : (kn >> 1) & 7) ^ hh) << 4);
+        const unsigned base = k_at + (i & (kStages - 1)) * kTile;
         // Groups of four fragments, of both halves of the tile, each read while the
         // one before is multiplied.
         V8 kf[2][4];
         const auto read_k = [&](int g) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                kf[g & 1][j] = *reinterpret_cast<const V8*>(kb + (j & 1) * 32 * kRow + (kat ^ ((2 * g + (j >> 1)) << 5)));
+                kf[g & 1][j] = *(const __attribute__((address_space(3))) V8*)((base ^ ((2 * g + (j >> 1)) << 5)) + (j & 1) * 32 * kRow);
         };
         read_k(0);
 #pragma unroll
@@ -781,79 +786,44 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
         }
         __builtin_amdgcn_sched_barrier(0);
     };
-    const auto weigh = [&](int i) {
-        const int stage = i & (kStages - 1), k0 = tile_key(i);
-        const bool mine = i >= np;
-        const char* vb = lds.v[stage];
-        // transposed read: lane 4 e + x of 16 holds row e's columns 4 x .., and lane
-        // i gets column i of the four rows
-        const int ln = here(lane), vrow = 4 * (ln >> 5) + ((ln & 15) >> 2), vsw = kRow == 256 ? vrow & 3 : (vrow >> 1) & 1;
-        const int vat = vrow * kRow + ((2 * ((ln >> 4) & 1) + ((ln & 3) >> 1)) << 4) + (ln & 1) * 8;
-        V8 vf[2][DB];
-        const auto read_v = [&](int g) {
+    V8 p[2][2];  // the weights of the tile before, whose second product is still to come
+    // O^T += V^T P^T of tile i, a product at a time, in four groups of fragments of
+    // which each is read while the one before is multiplied.
+    V8 vf[2][DB];
+    // transposed read: lane 4 e + x of 16 holds row e's columns 4 x .., and lane i
+    // gets column i of the four rows
+    const int vrow = 4 * hh + ((lane & 15) >> 2), vsw = kRow == 256 ? vrow & 3 : (vrow >> 1) & 1;
+    const unsigned v_at = lds_v + vrow * kRow + ((vsw << 6) | ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) << 4)) + (lane & 1) * 8;
+    const auto read_v = [&](int i, int g) {
+        const unsigned base = v_at + (i & (kStages - 1)) * kTile;
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                const char* at = vb + 16 * g * kRow + vat + ((d ^ vsw) << 6);
-                const s4 lo = read_tr(at), hi = read_tr(at + 8 * kRow);
-                vf[g & 1][d] = __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-            }
-        };
-        const unsigned long long ok = uniform(lds.there[i & (kFound - 1)]);
-        if (ok != ~0ull || (mine && k0 + kWideKeys > wave_min)) {
-            const int see = mine ? lim - k0 : kWideKeys;
-            unsigned long long there = ok & (see >= kWideKeys ? ~0ull : (see <= 0 ? 0ull : (1ull << see) - 1));
-            there >>= 4 * hh;
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int x = 0; x < 16; ++x)
-                    s[b][x] = (unsigned)(there >> 32 * b) & (1u << (8 * (x >> 2) + (x & 3))) ? s[b][x] : -INFINITY;
+        for (int d = 0; d < DB; ++d) {
+            const unsigned at = (base ^ (d << 6)) + 16 * g * kRow;
+            const s4 lo = read_tr(at), hi = read_tr(at + 8 * kRow);
+            vf[g & 1][d] = __builtin_bit_cast(V8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
-        float mx = s[0][0];
-#pragma unroll
-        for (int x = 1; x < 16; ++x) mx = fmaxf(mx, s[0][x]);
-#pragma unroll
-        for (int x = 0; x < 16; ++x) mx = fmaxf(mx, s[1][x]);
-        mx = fmaxf(mx, half_swap(mx));
-        const float mn = fmaxf(m, mx * a.scale);
-        // m only has to be near the largest score: weights up to 2^kSlack fit every type
-        if (__any(mn > m + kSlack)) {
-            const float alpha = __builtin_amdgcn_exp2f(m - finite_max(mn));
-            l *= alpha;
-#pragma unroll
-            for (int d = 0; d < DB; ++d) o[d] *= alpha;
-            m = mn;
-        }
-        const float ms = finite_max(m);
-        V8 p[2][2];
-        float sum = 0.0f;
-        read_v(0);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][x], a.scale, -ms));
-                sum = sum + e;
-                p[b][x >> 3][x & 7] = (T)e;
-            }
-        l = summed(l + sum);
+    };
+    const auto product = [&](int i) {
+        read_v(i, 0);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             __builtin_amdgcn_sched_barrier(0);
-            if (g < 3) read_v(g + 1);
+            if (g < 3) read_v(i, g + 1);
 #pragma unroll
             for (int d = 0; d < DB; ++d) o[d] = Mfma16<T>::dot32(vf[g & 1][d], p[g >> 1][g & 1], o[d]);
         }
         __builtin_amdgcn_sched_barrier(0);
-        // A key that only some rows see must not reach the others: what patch() cleared is
-        // added to the rows that do.
-        unsigned long long poison = mine && k0 + kWideKeys > min_lim ? __ballot(lds.poison[i & (kFound - 1)][lane] != 0) : 0;
-        for (; poison; poison &= poison - 1) {
-            const int kk = __builtin_ctzll(poison), at = ((kk >> 3) & 3) * 4 + (kk & 3), key = k0 + kk;
+    };
+    // A key that only some rows see must not reach the others: what patch() cleared in
+    // tile i is added to the rows that do.
+    const auto add_cleared = [&](int i) {
+        const int k0 = tile_key(i);
+        if (i < np || k0 + kWideKeys <= min_lim) return;
+        for (unsigned long long poison = __ballot(lds.poison[i & (kFound - 1)][lane] != 0); poison; poison &= poison - 1) {
+            const int kk = __builtin_ctzll(poison), at = (kk >> 5) * 16 + ((kk >> 3) & 3) * 4 + (kk & 3), key = k0 + kk;
             float pk = 0.0f;
 #pragma unroll
-            for (int x = 0; x < 16; ++x) pk = x == at ? (float)(kk < 32 ? p[0][x >> 3][x & 7] : p[1][x >> 3][x & 7]) : pk;
+            for (int x = 0; x < 32; ++x) pk = x == at ? (float)p[x >> 4][(x >> 3) & 1][x & 7] : pk;
             pk = __shfl(pk, (kk & 4) * 8 + n);
             const KeyPlace place = key_place(a.map, key, own.hi);
             const T* row = vp + key_offset(a.map, place, own.table[place.entry], key, own.hi);  // there, or it would be zeros
@@ -876,34 +846,120 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
             }
         }
     };
+    // The weights of tile i from its scores; beside their exponentials (ahead) the
+    // product of the tile before, an eighth of them to two products.
+    const auto weigh = [&](int i, auto ahead) {
+        constexpr bool kAhead = decltype(ahead)::value;
+        const int k0 = tile_key(i);
+        const bool mine = i >= np;
+        const unsigned long long ok = uniform(lds.there[i & (kFound - 1)]);
+        if (ok != ~0ull || (mine && k0 + kWideKeys > wave_min)) {
+            const int see = mine ? lim - k0 : kWideKeys;
+            unsigned long long there = ok & (see >= kWideKeys ? ~0ull : (see <= 0 ? 0ull : (1ull << see) - 1));
+            there >>= 4 * hh;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int x = 0; x < 16; ++x)
+                    s[b][x] = (unsigned)(there >> 32 * b) & (1u << (8 * (x >> 2) + (x & 3))) ? s[b][x] : -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int x = 1; x < 16; ++x) mx = fmaxf(mx, s[0][x]);
+#pragma unroll
+        for (int x = 0; x < 16; ++x) mx = fmaxf(mx, s[1][x]);
+        mx = fmaxf(mx, half_swap(mx));
+        const float mn = fmaxf(m, mx * a.scale);
+        V8 e[2][2];
+        float sum = 0.0f;
+        const auto eighth = [&](int z, float ms) {
+#pragma unroll
+            for (int y = 4 * z; y < 4 * z + 4; ++y) {
+                const int b = y >> 4, x = y & 15;
+                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][x], a.scale, -ms));
+                sum = sum + v;
+                e[b][x >> 3][x & 7] = (T)v;
+            }
+        };
+        // m only has to be near the largest score: weights up to 2^kSlack fit every
+        // type.  It is a whole number, so that what is scaled stays exact.
+        if (__any(mn > m + kSlack)) {
+            const float next = __builtin_ceilf(mn), alpha = __builtin_amdgcn_exp2f(m - finite_max(next));
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] *= alpha;
+            if constexpr (kAhead) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) p[b][u][x] = (T)((float)p[b][u][x] * alpha);
+            }
+            m = next;
+        }
+        const float ms = finite_max(m);
+        if constexpr (kAhead) {
+            read_v(i - 1, 0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                if (g < 3) read_v(i - 1, g + 1);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    o[d] = Mfma16<T>::dot32(vf[g & 1][d], p[g >> 1][g & 1], o[d]);
+                    if (d == 0) eighth(2 * g, ms);
+                    if (d == DB / 2) eighth(2 * g + 1, ms);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int z = 0; z < 8; ++z) eighth(z, ms);
+        }
+        l = summed(l + sum);
+        if constexpr (kAhead) add_cleared(i - 1);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) p[b][u] = e[b][u];
+    };
 
-    const bool late = w >= kWideWaves / 2;
     for (int i = 0; i < 3 && i < nt; ++i) {
         if (enter(i)) lds_barrier();
         if (w == i) find(i);
     }
     lds_barrier();
     for (int i = 0; i < 2 && i < nt; ++i) send(i);
-    // the same barriers either way
-    const auto tiles = [&](auto second) {
-        constexpr bool kLate = decltype(second)::value;
-        for (int i = 0; i <= nt; ++i) {
-            if (i + 1 < nt) wait_transfers<2 * NI>();  // all but the next tile's
-            else wait_transfers<0>();
-            if (i < nt) patch(i);
-            if (i + 3 < nt) enter(i + 3);
-            lds_barrier();  // tile i is there for all, tile i - 2 done with
-            if (i + 2 < nt) send(i + 2);
-            if (i + 3 < nt && w == (i & (kWideWaves - 1))) find(i + 3);
-            if (kLate && i > 0 && active(i - 1)) weigh(i - 1);
-            if (i < nt && active(i)) {
-                scores(i);
-                if (!kLate) weigh(i);
-            }
-        }
+    const auto wait_for = [&](int i) {
+        if (i + 1 < nt) wait_transfers<2 * NI>();  // all but the next tile's
+        else wait_transfers<0>();
+        patch(i);
+        if (i + 3 < nt) enter(i + 3);
+        lds_barrier();  // tile i is there for all, tile i - 2 done with
     };
-    if (late) tiles(std::true_type());
-    else tiles(std::false_type());
+    const auto send_ahead = [&](int i) {
+        if (i + 2 < nt) send(i + 2);
+        if (i + 3 < nt && w == (i & (kWideWaves - 1))) find(i + 3);
+    };
+    if (!wave_valid) {
+        for (int i = 0; i < nt; ++i) {
+            wait_for(i);
+            send_ahead(i);
+        }
+    } else if (nt > 0) {
+        wait_for(0);
+        scores(0);
+        send_ahead(0);
+        weigh(0, std::false_type());
+        for (int i = 1; i < nt; ++i) {
+            wait_for(i);
+            scores(i);
+            send_ahead(i);
+            weigh(i, std::true_type());
+        }
+        product(nt - 1);
+        add_cleared(nt - 1);
+    }
     lds_barrier();
 
     l = l + half_swap(l);
