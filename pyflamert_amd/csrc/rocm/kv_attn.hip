@@ -60,10 +60,22 @@ Plan plan(int num_cu, bool half,  int64_t max_added, int64_t max_length, int64_t
     p.own = kind(own_rows);
     a.whole = a.B > 0 && p.own == kWide && rows >= kWideRows * a.B && a.prefix_len + room < INT32_MAX - 4096;
     if (a.whole) {
+        const int64_t tiles = rows / kWideRows + a.B + 2;
         a.o_tiles = (int32_t)ceil_div(own_rows, kWideRows);
-        const int64_t tiles = a.Hkv * (rows / kWideRows + a.B);
-        split_keys(tiles >= num_cu ? 1 : ceil_div(num_cu, tiles), wide_round, a.prefix_len + max_length, &a.o_splits, &a.o_chunk);
-        if (a.o_splits == 0) a.o_splits = 1;
+        a.o_splits = 1;
+        a.o_chunk = INT32_MAX;
+        // Where a CU has few tiles, in equal shares of one workgroup a CU; with
+        // many, a tile to a workgroup and no scratch.
+        if (a.B + 2 <= kShareGroups && tiles * a.Hkv < 8 * num_cu) {
+            p.own = kShares;
+            a.shares = num_cu > a.Hkv ? num_cu / a.Hkv : 1;
+            a.items = (int32_t)tiles;
+            // parts as memory goes: 256 MB of them, at least three
+            const int64_t parts = (int64_t(256) << 20) / ((int64_t)a.T * a.Hq * a.D * 4);
+            a.parts = (int32_t)(parts < 3 ? 3 : (parts > kMaxParts ? kMaxParts : parts));
+            p.own_blocks = (int64_t)a.shares * a.Hkv;
+            return p;
+        }
     } else {
         p.prefix = kind(rows);
         if (a.B > 0 && p.prefix != kWide && p.own != kWide) p.prefix = p.own = p.prefix > p.own ? p.prefix : p.own;
@@ -183,24 +195,26 @@ void attention_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* q, pfr_dtype dtyp
     if (max_length == 0 || max_length > room) max_length = room;
     const Plan p = plan(ctx->num_cu, dtype != PFR_F32, max_added, max_length, room, a);
 
-    const int64_t parts = a.p_splits + a.o_splits, rows = T * heads;
-    if (!a.whole || parts > 1) {
+    const bool in_shares = p.own == pfr::attn::kShares;
+    const int64_t parts = in_shares ? a.parts : a.p_splits + a.o_splits, rows = T * heads;
+    if (!a.whole || in_shares) {
         const size_t o = (size_t)(parts * rows * kv->dim) * sizeof(float);
         char* ws = static_cast<char*>(ctx->scratch[7].ensure(o + (size_t)(parts * rows) * sizeof(float2) + 16));
         a.part_o = reinterpret_cast<float*>(ws);
         a.part_ml = reinterpret_cast<float2*>(ws + o);
     }
-    a.zeros = zeros(ctx, a.Hkv * (B + 2));
+    a.zeros = zeros(ctx, a.Hkv * (in_shares ? a.items : B + 2));
     auto* arrived = reinterpret_cast<uint32_t*>(const_cast<char*>(a.zeros) + kZeros);
-    const bool one = p.prefix == p.own;
+    const bool one = p.prefix == p.own;  // (a call in shares has no launch for the prefix)
     const auto by = [](int64_t n) { return pfr::FastDiv((uint32_t)(n > 0 ? n : 1)); };
     a.by_heads = by(a.Hkv);
     a.by_p_tiles = by(a.p_tiles);
     a.by_o_tiles = by(a.o_tiles);
+    a.by_fours = by(a.D / 4);
     a.by_requests = by(a.B + (a.whole ? 2 : 0));
     // the workgroups that come last join the rows, where few enough requests share the prefix's
     if (a.part_o != nullptr && p.own != pfr::attn::kWide && p.own_blocks > 0 &&
-        (!one || (B + 2 <= 64 && T * a.G <= 64)))
+        (in_shares || !one || (B + 2 <= 64 && T * a.G <= 64)))
         a.arrived = arrived;
     a.p_items = (int32_t)p.prefix_blocks;
     enqueue(ctx, kv, dtype, a, p.prefix, p.prefix_blocks + (one ? p.own_blocks : 0));

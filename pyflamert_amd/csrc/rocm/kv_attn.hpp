@@ -53,21 +53,22 @@ struct Args {
     // Apart: p_items = Hkv * p_tiles * p_splits workgroups for the prefix, p_chunk
     // keys a split, its tiles over the rows of all tokens; then Hkv * B *
     // o_tiles * o_splits for the requests' own keys, o_chunk a split.
-    // Together (whole): a request's tiles see the prefix and then its own
-    // keys; splits are of that whole range.
-    FastDiv by_heads, by_p_tiles, by_o_tiles, by_requests;
+    // Together (whole, and in shares): a request's tiles see the prefix and then
+    // its own keys.
+    FastDiv by_heads, by_p_tiles, by_o_tiles, by_requests, by_fours;  // by_fours: by D / 4
+    int32_t shares, parts, items;  // of a key head: workgroups, parts of a tile of rows at most, tiles at most
     int32_t whole, p_items, p_tiles, p_splits, p_chunk, o_tiles, o_splits, o_chunk;
     const char* zeros;  // 256 of them
     float* part_o;    // [p_splits + o_splits][T * Hq][D], null: rows are whole after one workgroup
     float2* part_ml;  // [p_splits + o_splits][T * Hq]: the score weighed against (log2 units), sum of weights
     // Arrivals at each key head's requests (and at the tokens of none), zero
     // between launches: the last workgroup joins the rows.  Null: a launch of its own does.
-    uint32_t* arrived;  // [Hkv][B + 2]
+    uint32_t* arrived;  // [Hkv][B + 2]; in shares [Hkv][items], by tile of rows
 };
 
 // The kernels: narrow (kNarrow1, 2: 16 or 32 rows, waves share the keys) and
-// wide (kWideRows rows, waves share a tile of keys).
-enum Kind { kNarrow1, kNarrow2, kWide };
+// wide (kWideRows rows, waves share a tile of keys), and wide in equal shares.
+enum Kind { kNarrow1, kNarrow2, kWide, kShares };
 
 template <class QT, class KT>
 void launch(hipStream_t s, const Args& a, Kind kind, unsigned blocks);
@@ -309,6 +310,11 @@ __device__ __forceinline__ float2 get_pair(const float2* p) {
     return make_float2(__builtin_bit_cast(float, (unsigned)v), __builtin_bit_cast(float, (unsigned)(v >> 32)));
 }
 
+// Four floats, the same way: a store of 16 bytes as the atomics' of eight.
+__device__ __forceinline__ void put_four(float* p, f4 x) {
+    asm volatile("global_store_dwordx4 %0, %1, off sc1" ::"v"(p), "v"(x) : "memory");
+}
+
 // A wave joins the parts of row R (query head R % Hq of token t): lane p holds part
 // p's statistics, and 32 lanes (64 past 128 columns) add up its values, two
 // parts at a time.  SHARED: the parts are of this launch.
@@ -411,7 +417,7 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
     // block before has its scores, its V as soon as that has its sums.
     // lane i (modulo a block) finds key i of a block: its table entry, and once that is there its offset
     constexpr int kB = kBlock<QT>, NJ = TT::NJ;
-    constexpr uint32_t kAll = kB == 32 ? ~0u : (1u << kB) - 1;
+    constexpr uint32_t kAll = ~0u >> (32 - kB);
     constexpr int step = kWaves * kB;
     const int first = lo + w * kB;
     const auto find = [&](int k0) { return key_place(a.map, k0 + (lane & (kB - 1)), hi); };
@@ -612,9 +618,10 @@ struct WideLds {
 
 // 16 bytes a lane from memory to the LDS, lane i's to byte lds + 16 i.  The
 // compiler does not see these transfers: every read behind them has to wait
-// for them by hand, and no wait that it places counts them.
+// for them by hand, and no wait that it places counts them.  (m0 is set by
+// whatever uses it.)
 __device__ __forceinline__ void transfer(const void* from, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
 }
 template <int N>
 __device__ __forceinline__ void wait_transfers() {  // until at most N of the wave's are left
@@ -625,13 +632,14 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // Rows r0 .. of the n_rows that start at token t0 (see narrow) against the keys of
 // pre, which all of them see, and then those of own, of which row r sees the
 // ones below lim0 + r / G.  part < 0: nothing else has a part in these rows.
+// SHARED: another workgroup of this launch may read the part.
 //
 // Tiles of 64 keys come to the LDS two tiles ahead, every wave moving its share
 // past the registers; a wave multiplies them with its 32 rows as S^T = K Q^T
 // and O^T = V^T P^T in 32x32x16 products, so that a row's scores, its weights
 // and its column of O^T stay in the lanes n and n + 32.  The second product of
 // a tile runs beside the exponentials of the next.
-template <class T, int DP, bool FULL>
+template <class T, int DP, bool FULL, bool SHARED>
 __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int t0, int r0, int n_rows, const Seg& pre,
                                      const Seg& own, int lim0, int part) {
     typedef typename Mfma16<T>::V8 V8;
@@ -986,7 +994,7 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
         return;
     }
     const int64_t at = (int64_t)part * a.T * a.Hq + R;
-    if (eh == 0) a.part_ml[at] = make_float2(m, l);
+    if (eh == 0) put_pair(a.part_ml + at, m, l);
     float* row = a.part_o + at * a.D;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -994,10 +1002,9 @@ __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int
         for (int j = 0; j < 4; ++j) {
             const int c = 32 * d + 8 * j + 4 * eh;
             if (FULL || c < a.D) {
-                f4 x;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = o[d][4 * j + e];
-                *reinterpret_cast<f4*>(row + c) = x;
+                const f4 x = {o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+                if constexpr (SHARED) put_four(row + c, x);
+                else *reinterpret_cast<f4*>(row + c) = x;
             }
         }
 }
@@ -1122,7 +1129,7 @@ __device__ __forceinline__ void attention(const Args& a, char* lds) {
         const Seg pre{a.prefix_table, lo < P ? lo : P, hi < P ? hi : P};
         const Seg own{table, lo > P ? lo - P : 0, hi > P ? hi - P : 0};
         if constexpr (DW > 0) {
-            wide<QT, DW, WF>(a, *reinterpret_cast<WideLds<DW>*>(lds), x.h, t0, r0, n_rows, pre, own, lim0, part);
+            wide<QT, DW, WF, false>(a, *reinterpret_cast<WideLds<DW>*>(lds), x.h, t0, r0, n_rows, pre, own, lim0, part);
         } else {
             narrow<QT, KT, DN, RT, FULL>(a, reinterpret_cast<float*>(lds), x.h, t0, r0, n_rows, prefix ? pre : own, lim0, prefix ? 0 : 1, part);
             __syncthreads();
@@ -1134,6 +1141,198 @@ __device__ __forceinline__ void attention(const Args& a, char* lds) {
             // without a prefix nothing else comes to the tokens of no request
             if (a.p_splits == 0 && x.b == 0 && x.tile == 0 && x.split == 0)
                 for (int b = a.B; b < a.B + 2; ++b) join_rows<QT>(a, x.h, b);
+        }
+    }
+}
+
+// ---- prompts: equal shares of the wide form's work ------------------------------------
+
+constexpr int kShareGroups = kWideWaves * 64;  // requests, and the two runs of tokens of none, a thread each
+
+struct ShareLds {
+    int64_t units[kShareGroups + 1];  // units before each request's
+    int32_t tiles[kShareGroups + 1];
+    int64_t wave_units[kWideWaves];
+    int32_t wave_tiles[kWideWaves], wave_most[kWideWaves];
+    int32_t last;
+};
+
+// The rows of request b (or of none, b = B and B + 1) and the keys they see.
+struct Rows {
+    int t0, n_rows, lim0;
+    int64_t room;
+    const int32_t* table;
+};
+__device__ __forceinline__ Rows rows_of(const Args& a, int b) {
+    Rows q;
+    int t1;
+    tokens_of(a.start, a.B, b, a.T, &q.t0, &t1);
+    q.n_rows = (t1 - q.t0) * a.G;
+    q.lim0 = 0;
+    q.room = 0;
+    q.table = nullptr;
+    if (b < a.B) {
+        q.lim0 = first_limit(a.lengths[b], t1 - q.t0);
+        q.room = (int64_t)a.table_w * a.map.page.d;
+        q.table = a.table + (int64_t)b * a.table_ld;
+    }
+    return q;
+}
+// Keys of a tile of rows: the prefix, and the own ones that its last row sees; and
+// its units, tiles of keys, one at least, for its rows have to be written.
+__device__ __forceinline__ int tile_keys(const Args& a, const Rows& q, int tile) {
+    const int r1 = (tile + 1) * kWideRows < q.n_rows ? (tile + 1) * kWideRows : q.n_rows;
+    return a.prefix_len + keys_end(q.lim0, (int)a.group.div((uint32_t)(r1 - 1)), q.room);
+}
+__device__ __forceinline__ int units_of(int keys) { return keys > kWideKeys ? (keys + kWideKeys - 1) / kWideKeys : 1; }
+
+// The workgroup joins `parts` parts of rows [r0, r1): their weights by row, then
+// four columns a thread.
+template <class T>
+__device__ __forceinline__ void join_tile(const Args& a, float* weight, int h, int t0, int r0, int r1, int parts) {
+    typedef T T4 __attribute__((ext_vector_type(4), aligned(2)));
+    const int64_t rows = (int64_t)a.T * a.Hq;
+    const auto row_of = [&](int r, int* t, int* hq) {
+        const int dt = (int)a.group.div((uint32_t)r);
+        *t = t0 + dt;
+        *hq = h * a.G + r - dt * a.G;
+    };
+    for (int r = r0 + (int)threadIdx.x; r < r1; r += (int)blockDim.x) {
+        int t, hq;
+        row_of(r, &t, &hq);
+        const float2* ml = a.part_ml + (int64_t)t * a.Hq + hq;
+        float M = -INFINITY, L = 0.0f;
+        for (int p = 0; p < parts; ++p) M = fmaxf(M, get_pair(ml + p * rows).x);
+        for (int p = 0; p < parts; ++p) {
+            const float2 x = get_pair(ml + p * rows);
+            const float f = x.x == -INFINITY && x.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x.x - finite_max(M));
+            if (f != 0.0f) L = L + f * x.y;
+            weight[p * kWideRows + r - r0] = f;
+        }
+        for (int p = 0; p < parts; ++p) weight[p * kWideRows + r - r0] = L == 0.0f ? 0.0f : weight[p * kWideRows + r - r0] / L;
+    }
+    __syncthreads();
+    const int n = (r1 - r0) * (a.D / 4);
+#pragma unroll 4
+    for (int z = (int)threadIdx.x; z < n; z += kWideWaves * 64) {
+        const int r = (int)a.by_fours.div((uint32_t)z), d = 4 * (z - r * (a.D / 4));
+        int t, hq;
+        row_of(r0 + r, &t, &hq);
+        const float* src = a.part_o + ((int64_t)t * a.Hq + hq) * a.D + d;
+        f4 acc = f4(0.0f);
+        for (int p = 0; p < parts; ++p) {
+            const float2* at = reinterpret_cast<const float2*>(src + p * rows * a.D);
+            const float2 u = get_pair(at), v = get_pair(at + 1);
+            const float f = weight[p * kWideRows + r];
+            acc[0] = acc[0] + f * u.x;
+            acc[1] = acc[1] + f * u.y;
+            acc[2] = acc[2] + f * v.x;
+            acc[3] = acc[3] + f * v.y;
+        }
+        T4 x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = (T)acc[e];
+        *reinterpret_cast<T4*>(static_cast<T*>(a.out) + (int64_t)t * a.ldo + (int64_t)hq * a.D + d) = x;
+    }
+    __syncthreads();
+}
+
+// A key head's tiles of rows, each with the prefix and then its request's own
+// keys, laid end to end in units of 64 keys and cut into equal shares, one a
+// workgroup: with a tile to a workgroup, 2.2 tiles to a CU took as long as
+// three.  A tile that is cut is joined by the workgroup that comes last to it.
+template <class T, int DW, bool WF>
+__device__ __forceinline__ void shares(const Args& a, WideLds<DW>& lds, ShareLds& sh) {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, nb = a.B + 2;
+    const int j = (int)a.by_heads.div(blockIdx.x), h = (int)blockIdx.x - j * a.Hkv;
+    int64_t units = 0;
+    int tiles = 0, most = 0;
+    if (tid < nb) {
+        const Rows q = rows_of(a, tid);
+        tiles = (q.n_rows + kWideRows - 1) / kWideRows;
+        for (int t = 0; t < tiles; ++t) {
+            const int u = units_of(tile_keys(a, q, t));
+            units += u;
+            most = u > most ? u : most;
+        }
+    }
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t x = __shfl_up(units, o);
+        const int y = __shfl_up(tiles, o), z = __shfl_xor(most, o);
+        if (lane >= o) {
+            units += x;
+            tiles += y;
+        }
+        most = z > most ? z : most;
+    }
+    if (lane == 63) {
+        sh.wave_units[w] = units;
+        sh.wave_tiles[w] = tiles;
+        sh.wave_most[w] = most;
+    }
+    if (tid == 0) {
+        sh.units[0] = 0;
+        sh.tiles[0] = 0;
+    }
+    __syncthreads();
+    int64_t all = 0;
+    for (int i = 0; i < kWideWaves; ++i) {
+        if (i < w) {
+            units += sh.wave_units[i];
+            tiles += sh.wave_tiles[i];
+        }
+        all += sh.wave_units[i];
+        most = sh.wave_most[i] > most ? sh.wave_most[i] : most;
+    }
+    sh.units[tid + 1] = units;
+    sh.tiles[tid + 1] = tiles;
+    __syncthreads();
+    // a tile in `most` units meets at most parts workgroups
+    int64_t share = (all + a.shares - 1) / a.shares;
+    const int64_t least = (most + a.parts - 2) / (a.parts - 1);
+    share = share < least ? least : share;
+    const int64_t u0 = (int64_t)uniform((unsigned long long)(j * share)), u1 = u0 + share < all ? u0 + share : all;
+    if (u0 >= u1) return;
+    int b = 0;
+    for (int hi = nb; hi - b > 1;) {
+        const int mid = (b + hi) >> 1;
+        if (sh.units[mid] <= u0) b = mid;
+        else hi = mid;
+    }
+    b = uniform(b);
+    int64_t c = (int64_t)uniform((unsigned long long)sh.units[b]);
+    for (; b < nb && c < u1; ++b) {
+        Rows q = rows_of(a, b);
+        q.t0 = uniform(q.t0);
+        q.n_rows = uniform(q.n_rows);
+        q.lim0 = uniform(q.lim0);
+        for (int tile = 0; tile * kWideRows < q.n_rows && c < u1; ++tile) {
+            const int keys = uniform(tile_keys(a, q, tile)), n = units_of(keys);
+            const int64_t next = c + n;
+            if (next > u0) {
+                const int from = u0 > c ? (int)(u0 - c) : 0, to = u1 < next ? (int)(u1 - c) : n;
+                const int lo = from * kWideKeys, hi = to * kWideKeys < keys ? to * kWideKeys : keys, P = a.prefix_len;
+                const int j0 = (int)(c / share), j1 = (int)((next - 1) / share);
+                const int r0 = tile * kWideRows;
+                const Seg pre{a.prefix_table, lo < P ? lo : P, hi < P ? hi : P};
+                const Seg own{q.table, lo > P ? lo - P : 0, hi > P ? hi - P : 0};
+                wide<T, DW, WF, true>(a, lds, h, q.t0, r0, q.n_rows, pre, own, q.lim0, j1 > j0 ? j - j0 : -1);
+                if (j1 > j0) {
+                    __builtin_amdgcn_s_waitcnt(0);  // the wave's stores have reached their coherent home
+                    __syncthreads();
+                    if (tid == 0) {
+                        uint32_t* at = a.arrived + (int64_t)h * a.items + sh.tiles[b] + tile;
+                        const bool last = __hip_atomic_fetch_add(at, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(j1 - j0);
+                        if (last) __hip_atomic_store(at, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        sh.last = last;
+                    }
+                    __syncthreads();
+                    if (sh.last)
+                        join_tile<T>(a, reinterpret_cast<float*>(lds.k), h, q.t0, r0,
+                                     r0 + kWideRows < q.n_rows ? r0 + kWideRows : q.n_rows, j1 - j0 + 1);
+                }
+            }
+            c = next;
         }
     }
 }
@@ -1155,10 +1354,18 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void k_attn_wide(Args a) {
     attention<T, T, 64, false, 1, DW, WF>(a, lds);
 }
 
+template <class T, int DW, bool WF>
+__global__ __launch_bounds__(kWideWaves * 64, 2) void k_attn_shares(Args a) {
+    __shared__ WideLds<DW> lds;
+    __shared__ ShareLds sh;
+    shares<T, DW, WF>(a, lds, sh);
+}
+
 template <class QT, class KT, int DN, bool FULL, int DW, bool WF>
 void launch_kind(hipStream_t s, const Args& a, Kind kind, unsigned blocks) {
     const dim3 grid(blocks), wg(kWaves * 64);
     if constexpr (DW > 0) {
+        if (kind == kShares) { hipLaunchKernelGGL((k_attn_shares<QT, DW, WF>), grid, dim3(kWideWaves * 64), 0, s, a); return; }
         if (kind == kWide) { hipLaunchKernelGGL((k_attn_wide<QT, DW, WF>), grid, dim3(kWideWaves * 64), 0, s, a); return; }
     }
     if constexpr (DN < 256) {

@@ -265,6 +265,15 @@ SHAPES = {
     "wide heads": (4, 2, 256, 16, "head", 70, [20, 45], [1, 9]),
     "wide odd heads": (2, 2, 200, 16, "token", 33, [20, 35], [1, 2]),
     "long": (2, 1, 128, 16, "head", 3000, [1500, 700], [1, 1]),
+    "rows of one tile and a bit": (20, 1, 128, 16, "head", 90, [40, 7], [1, 1]),
+    "prefix of many rows": (8, 2, 128, 16, "head", 700, [9, 1, 40, 33] * 6, [1] * 24),
+    "prefix of many rows, odd dim": (6, 1, 72, 7, "token", 333, [9, 1, 40, 33] * 3, [1] * 12),
+    "prefix and own keys of many rows": (8, 1, 64, 16, "token", 1100, [40, 330, 25], [9, 6, 30]),
+    "many rows a request": (8, 1, 64, 16, "head", 130, [230, 95], [200, 90]),
+    "many rows a request, odd dim": (4, 2, 80, 24, "token", 70, [250, 180], [250, 170]),
+    "many rows a request, no prefix": (8, 1, 128, 16, "head", 0, [130, 200], [130, 100]),
+    "many rows a request, longer than a window": (16, 1, 96, 1, "head", 2500, [90, 1300], [30, 20]),
+    "one long request": (4, 1, 128, 16, "head", 200, [900, 5, 3], [300, 4, 1]),
 }
 
 
@@ -297,6 +306,48 @@ def test_attention_rows_without_keys(ctx, q, cache, how):
     c.check(ctx)
     c.start, c.lengths, c.table = np.zeros(1, np.int32), np.zeros(0, np.int32), np.zeros((0, 1), np.int32)
     c.check(ctx)
+
+
+@pytest.mark.parametrize("q,cache", TYPES[:2])
+def test_attention_of_many_rows_where_keys_are_missing(ctx, q, cache):
+    """Rows without keys, tokens of no request and pages outside the pool, where a
+    request has many rows."""
+    c = Case(8, 1, 64, 16, "head", q, cache, 0, [0, 60, 90], [40, 100, 30])
+    got = c.check(ctx)
+    assert bool((got[:40] == 0).all()) and bool((got[40:80] == 0).all())  # 60 keys of 100 tokens: 40 before the first
+    for prefix in (0, 150):
+        c = Case(8, 1, 128, 16, "token", q, cache, prefix, [130, 90, 33], [100, 60, 20])
+        c.table[0, 1] = -1
+        c.table[1, :] = 2 ** 31 - 1
+        if prefix:
+            c.prefix_table[2] = c.kp.shape[0]
+        c.check(ctx)
+        # the last request's tokens are of none; then the first 100 as well
+        c.lengths, c.table, c.start = c.lengths[:2], c.table[:2], c.start[:3].copy()
+        c.check(ctx)
+        c.lengths, c.table, c.start = c.lengths[1:], c.table[1:], c.start[1:].copy()
+        c.check(ctx)
+
+
+@pytest.mark.parametrize("q,cache", TYPES[:2])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_attention_of_many_rows_later_keys(ctx, q, cache, value):
+    """An infinity or a NaN in a late value reaches the tokens that see it, in its
+    column, and no others, across tiles of rows and of keys."""
+    def case():
+        return Case(8, 1, 128, 16, "head", q, cache, 40, [290, 9], [260, 3])
+
+    clean = case().run(ctx)
+    for key in (31, 64, 200, 289):  # token key - 30 of request 0 is the first that sees it
+        c = case()
+        p, off = c.slot_of(0, key)
+        c.vp[p, :, off, 77] = value
+        got = c.run(ctx)
+        first = key - 30
+        assert torch.equal(bits(got[:first]), bits(clean[:first])) and torch.equal(bits(got[260:]), bits(clean[260:]))
+        assert bool((~torch.isfinite(got[first:260, :, 77])).all())
+        rest = torch.arange(128) != 77
+        assert torch.equal(bits(got[first:260][..., rest]), bits(clean[first:260][..., rest]))
 
 
 @pytest.mark.parametrize("q,cache", TYPES[:4])
