@@ -85,15 +85,13 @@ __device__ __forceinline__ void block_sum(int64_t& x, int64_t& y, int& bits, int
     __syncthreads();
 }
 
-// The last entry of the ascending s[0 .. n) that is <= v (s[0] <= v).
-__device__ __forceinline__ int last_at_most(const int64_t* s, int n, int64_t v) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (s[mid] <= v) lo = mid;
-        else hi = mid;
-    }
-    return lo;
+// The last of the ascending s[0 .. kTabThreads) that is <= v (s[0] <= v).
+__device__ __forceinline__ int last_at_most(const int64_t* s, int64_t v) {
+    int at = 0;
+#pragma unroll
+    for (int step = kTabThreads / 2; step; step >>= 1)
+        if (s[at + step] <= v) at += step;
+    return at;
 }
 
 // Grid (groups of kTabThreads requests) x (slices of a group's tokens and new
@@ -109,8 +107,15 @@ __global__ __launch_bounds__(kTabThreads) void k_kv_tables(TablesArgs a) {
     const int r0 = (int)blockIdx.x * kTabThreads;
     const bool last_group = blockIdx.x + 1 == gridDim.x;
 
+    // every load that waits for nothing first
+    const int r = r0 + tid;
+    const bool mine = r < a.B;
+    const int32_t cached = mine ? a.cached[r] : 0, added = mine ? a.added[r] : 0;
+    int32_t head = a.head != nullptr ? *a.head : 0;
+
     int64_t tok0 = 0, pg0 = 0;
     int bits = 0;
+#pragma unroll 4
     for (int r = tid; r < r0; r += kTabThreads) {
         const Need n = need_of(a, a.cached[r], a.added[r]);
         tok0 += n.added;
@@ -119,10 +124,8 @@ __global__ __launch_bounds__(kTabThreads) void k_kv_tables(TablesArgs a) {
     }
     if (r0 > 0) block_sum(tok0, pg0, bits, red, redb);
 
-    const int r = r0 + tid;
-    const bool mine = r < a.B;
     Need n = {};
-    if (mine) n = need_of(a, a.cached[r], a.added[r]);
+    if (mine) n = need_of(a, cached, added);
     // inclusive scans over the group
     int64_t x = n.added, y = n.pages;
     for (int o = 1; o < 64; o <<= 1) {
@@ -149,7 +152,6 @@ __global__ __launch_bounds__(kTabThreads) void k_kv_tables(TablesArgs a) {
     __syncthreads();
     const int64_t n_tok = tok[kTabThreads], n_pg = pg[kTabThreads];
 
-    int32_t head = a.head != nullptr ? *a.head : 0;
     const bool bad_head = head < 0 || head > a.n_free;
     head = head < 0 ? 0 : (head > a.n_free ? a.n_free : head);
 
@@ -179,20 +181,33 @@ __global__ __launch_bounds__(kTabThreads) void k_kv_tables(TablesArgs a) {
     };
     const int64_t ny = gridDim.y, sl = blockIdx.y;
     const int64_t t_lo = n_tok * sl / ny, t_hi = n_tok * (sl + 1) / ny;
-    for (int64_t t = t_lo + tid; t < t_hi && tok0 + t < a.max_tokens; t += kTabThreads) {
-        const int q = last_at_most(tok, kTabThreads, t);
-        const uint32_t p = (uint32_t)s_cached[q] + (uint32_t)(t - tok[q]);
-        const uint32_t j = a.page.div(p), off = p - j * a.page.d;
-        int32_t id = -1;
-        if ((int64_t)j < a.table_w) {
-            if ((int32_t)j < s_have[q]) id = a.table[(int64_t)(r0 + q) * a.table_ld + j];
-            else id = taken_page(pg0 + pg[q] + (int32_t)j - s_have[q]);
+    // four tokens at a time, so that the pages of one are not waited for before the next is looked up
+    constexpr int kAtOnce = 4;
+    const int64_t t_end = tok0 + t_hi < a.max_tokens ? t_hi : a.max_tokens - tok0;
+    for (int64_t t0 = t_lo + tid; t0 < t_end; t0 += kAtOnce * kTabThreads) {
+        int64_t slot[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int64_t t = t0 + i * kTabThreads;
+            slot[i] = -1;
+            if (t >= t_end) continue;
+            const int q = last_at_most(tok, t);
+            const uint32_t p = (uint32_t)s_cached[q] + (uint32_t)(t - tok[q]);
+            const uint32_t j = a.page.div(p), off = p - j * a.page.d;
+            int32_t id = -1;
+            if ((int64_t)j < a.table_w) {
+                if ((int32_t)j < s_have[q]) id = a.table[(int64_t)(r0 + q) * a.table_ld + j];
+                else id = taken_page(pg0 + pg[q] + (int32_t)j - s_have[q]);
+            }
+            slot[i] = id < 0 ? -1 : (int64_t)id * a.page.d + off;
         }
-        a.slots[tok0 + t] = id < 0 ? -1 : (int64_t)id * a.page.d + off;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+            if (t0 + i * kTabThreads < t_end) a.slots[tok0 + t0 + i * kTabThreads] = slot[i];
     }
     const int64_t p_lo = n_pg * sl / ny, p_hi = n_pg * (sl + 1) / ny;
     for (int64_t p = p_lo + tid; p < p_hi; p += kTabThreads) {
-        const int q = last_at_most(pg, kTabThreads, p);
+        const int q = last_at_most(pg, p);
         const int64_t j = s_have[q] + (p - pg[q]);
         if (j < a.table_w) a.table[(int64_t)(r0 + q) * a.table_ld + j] = taken_page(pg0 + p);
     }
