@@ -1069,13 +1069,15 @@ __device__ __forceinline__ void arrive(const Args& a, int h, int b, unsigned lon
     __syncthreads();
     const int lane = threadIdx.x & 63, w = (int)threadIdx.x >> 6;
     if (w == 0) {
-        // lane i: request i, or the tokens of none (B, B + 1); up to 64 of them
+        // after the prefix lane i asks for request i, or the tokens of none (B, B +
+        // 1), up to 64 of them; else the first lane for the workgroup's own request
         bool last = false;
-        if (b < 0 ? lane < a.B + 2 : lane == b) {
+        const int mine = b < 0 ? lane : b;
+        if (b < 0 ? lane < a.B + 2 : lane == 0) {
             int t0, t1;
-            tokens_of(a.start, a.B, lane, a.T, &t0, &t1);
-            const uint32_t all = (a.p_items > 0 ? a.p_tiles * a.p_splits : 0) + (lane < a.B ? a.o_tiles * a.o_splits : 0);
-            uint32_t* at = a.arrived + h * (a.B + 2) + lane;
+            tokens_of(a.start, a.B, mine, a.T, &t0, &t1);
+            const uint32_t all = (a.p_items > 0 ? a.p_tiles * a.p_splits : 0) + (mine < a.B ? a.o_tiles * a.o_splits : 0);
+            uint32_t* at = a.arrived + (int64_t)h * (a.B + 2) + mine;
             last = t1 > t0 && __hip_atomic_fetch_add(at, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == all;
             if (last) __hip_atomic_store(at, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
@@ -1083,7 +1085,7 @@ __device__ __forceinline__ void arrive(const Args& a, int h, int b, unsigned lon
         if (lane == 0) *flags = mask;
     }
     __syncthreads();
-    for (unsigned long long mask = uniform(*flags); mask; mask &= mask - 1) join_rows<QT>(a, h, __builtin_ctzll(mask));
+    for (unsigned long long mask = uniform(*flags); mask; mask &= mask - 1) join_rows<QT>(a, h, b < 0 ? __builtin_ctzll(mask) : b);
 }
 
 // The narrow form (DN columns, FULL: all of them there, RT tiles of rows) or, with
@@ -1138,8 +1140,8 @@ __device__ __forceinline__ void attention(const Args& a, char* lds) {
     if constexpr (DW == 0) {
         if (a.arrived != nullptr) {
             if (n_rows > 0) arrive<QT>(a, x.h, x.b, reinterpret_cast<unsigned long long*>(lds));
-            // without a prefix nothing else comes to the tokens of no request
-            if (a.p_splits == 0 && x.b == 0 && x.tile == 0 && x.split == 0)
+            // nothing else of this launch comes to the tokens of no request
+            if (a.p_items == 0 && x.b == 0 && x.tile == 0 && x.split == 0)
                 for (int b = a.B; b < a.B + 2; ++b) join_rows<QT>(a, x.h, b);
         }
     }

@@ -267,6 +267,8 @@ SHAPES = {
     "long": (2, 1, 128, 16, "head", 3000, [1500, 700], [1, 1]),
     "rows of one tile and a bit": (20, 1, 128, 16, "head", 90, [40, 7], [1, 1]),
     "prefix of many rows": (8, 2, 128, 16, "head", 700, [9, 1, 40, 33] * 6, [1] * 24),
+    "many requests": (8, 1, 64, 16, "head", 300, [1 + 7 * i % 90 for i in range(100)], [1] * 100),
+    "many requests, no prefix": (2, 2, 128, 16, "token", 0, [1 + 7 * i % 90 for i in range(70)], [1] * 70),
     "prefix of many rows, odd dim": (6, 1, 72, 7, "token", 333, [9, 1, 40, 33] * 3, [1] * 12),
     "prefix and own keys of many rows": (8, 1, 64, 16, "token", 1100, [40, 330, 25], [9, 6, 30]),
     "many rows a request": (8, 1, 64, 16, "head", 130, [230, 95], [200, 90]),
