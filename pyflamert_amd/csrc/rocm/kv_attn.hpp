@@ -383,10 +383,11 @@ __device__ __forceinline__ s4 read_tr(unsigned lds) {
 // One workgroup's rows against keys [lo, hi) of one table.  Rows r0 .. of the
 // n_rows that start at token t0: row r is query head r % G of token t0 + r / G.
 // lim0 and per_token: row r sees keys below lim0 + per_token * (r / G).
-// Writes the rows' part `part`.
+// Writes the rows' part `part`.  found: id0 is the table's entry for the lane's key of
+// the wave's first block already.
 template <class QT, class KT, int DP, int RT, bool FULL>
 __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0, int r0, int n_rows,
-                                       const Seg& seg, int lim0, int per_token, int part) {
+                                       const Seg& seg, int lim0, int per_token, int part, bool found, int32_t id0) {
     const int32_t* __restrict__ table = seg.table;
     const int lo = seg.lo, hi = seg.hi;
     typedef Tiles<QT, KT, DP, RT, FULL> TT;
@@ -438,7 +439,7 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
     int32_t id1 = 0;
     if (first < hi) {
         const KeyPlace at = find(first);
-        const int32_t id = table[at.entry];
+        const int32_t id = found ? id0 : table[at.entry];
         at1 = find(first + step);
         id1 = table[at1.entry];
         off = offset(first, at, id);
@@ -1097,16 +1098,24 @@ __device__ __forceinline__ void attention(const Args& a, char* lds) {
     int t0 = 0, t1 = a.T, lim0 = a.prefix_len, P = a.prefix_len, part = x.split, tiles_apart = a.p_tiles;
     int64_t room = 0;
     const int32_t* table = nullptr;
+    int32_t id0 = 0;
+    int first = -1;
     if (!prefix) {
-        if (a.whole) tokens_of(a.start, a.B, x.b, a.T, &t0, &t1);
-        else request_tokens(a.start, x.b, a.T, &t0, &t1);
         const bool listed = x.b < a.B;  // else tokens of no request
-        lim0 = 0;
         if (listed) {
-            lim0 = first_limit(a.lengths[x.b], t1 - t0);
             room = (int64_t)a.table_w * a.map.page.d;
             table = a.table + (int64_t)x.b * a.table_ld;
         }
+        if (DW == 0 && (int64_t)x.split * a.o_chunk < room) {
+            // the first keys' entries, while the request's length is on its way
+            constexpr int kB = kBlock<QT>;
+            first = x.split * a.o_chunk;
+            const int w = (int)threadIdx.x >> 6, key = first + w * kB + ((int)threadIdx.x & (kB - 1));
+            id0 = table[key_place(a.map, key, (int)room).entry];
+        }
+        if (a.whole) tokens_of(a.start, a.B, x.b, a.T, &t0, &t1);
+        else request_tokens(a.start, x.b, a.T, &t0, &t1);
+        lim0 = listed ? first_limit(a.lengths[x.b], t1 - t0) : 0;
         t0 = uniform(t0);
         t1 = uniform(t1);
         lim0 = uniform(lim0);
@@ -1133,7 +1142,8 @@ __device__ __forceinline__ void attention(const Args& a, char* lds) {
         if constexpr (DW > 0) {
             wide<QT, DW, WF, false>(a, *reinterpret_cast<WideLds<DW>*>(lds), x.h, t0, r0, n_rows, pre, own, lim0, part);
         } else {
-            narrow<QT, KT, DN, RT, FULL>(a, reinterpret_cast<float*>(lds), x.h, t0, r0, n_rows, prefix ? pre : own, lim0, prefix ? 0 : 1, part);
+            narrow<QT, KT, DN, RT, FULL>(a, reinterpret_cast<float*>(lds), x.h, t0, r0, n_rows, prefix ? pre : own, lim0, prefix ? 0 : 1, part,
+                                         lo == first, id0);
             __syncthreads();
         }
     }
