@@ -310,9 +310,11 @@ __device__ __forceinline__ float2 get_pair(const float2* p) {
     return make_float2(__builtin_bit_cast(float, (unsigned)v), __builtin_bit_cast(float, (unsigned)(v >> 32)));
 }
 
-// Four floats, the same way: a store of 16 bytes as the atomics' of eight.
+// Four floats, the same way: a store of 16 bytes as the atomics' of eight.  Such a
+// store still reads its data for two wait states, which the compiler keeps for
+// its own stores but not behind an asm block.
 __device__ __forceinline__ void put_four(float* p, f4 x) {
-    asm volatile("global_store_dwordx4 %0, %1, off sc1" ::"v"(p), "v"(x) : "memory");
+    asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" ::"v"(p), "v"(x) : "memory");
 }
 
 // A wave joins the parts of row R (query head R % Hq of token t): lane p holds part
