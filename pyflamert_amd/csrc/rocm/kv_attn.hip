@@ -30,9 +30,6 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Splits of `keys` keys, each of `chunk` keys (a multiple of `round`), for
 // about `want` of them, and at most kMaxParts.
 constexpr int kMaxParts = 24;
-#ifndef EV
-#define EV(n, d) d
-#endif
 void split_keys(int64_t want, int64_t round, int64_t keys, int32_t* splits, int32_t* chunk) {
     int64_t s = ceil_div(keys, round);
     s = want < s ? want : s;
@@ -42,6 +39,14 @@ void split_keys(int64_t want, int64_t round, int64_t keys, int32_t* splits, int3
     *chunk = (int32_t)c;
 }
 
+// Own keys of so many blocks at most go to a wave each: with one to a workgroup,
+// 67 requests of one key, 32 heads, took 77 us, 36 so.
+constexpr int kSoloBlocks = 8;
+// Rows of a key head that the workgroups that come last join themselves; more
+// take a launch, for that joins them side by side (14 rows of 24 parts: 87 us
+// in the workgroups, 24 so; 4 rows of 5: 9 us, 12 so).
+constexpr int kJoinRows = 8;
+
 // The kernels of a call and their workgroups; one launch where both parts take the same kernel.
 struct Plan {
     Kind prefix = pfr::attn::kNarrow1, own = pfr::attn::kNarrow1;
@@ -49,13 +54,16 @@ struct Plan {
 };
 
 // Which kernels, and how the work is cut into workgroups.
-Plan plan(int num_cu, bool half,  int64_t max_added, int64_t max_length, int64_t room, Args& a) {
+Plan plan(int num_cu, bool half, int64_t max_added, int64_t max_length, int64_t room, Args& a) {
     using namespace pfr::attn;
     Plan p;
     const int64_t rows = (int64_t)a.T * a.G, own_rows = max_added * a.G;  // of a key head
-    const auto kind = [&](int64_t n) { return half && a.D <= 128 && n > 32 ? kWide : (a.D <= 128 && n > 16 ? kNarrow2 : kNarrow1); };
+    // Float32 rows go 16 to a wave however many they are: with 32 a wave's
+    // registers leave one workgroup to a CU where two hide each other's loads
+    // (64 requests, 8 heads of 96 for 64 of q, 2752 keys: 121 us with 32, 100 so).
+    const auto kind = [&](int64_t n) { return half && a.D <= 128 && n > 16 ? (n > 32 ? kWide : kNarrow2) : kNarrow1; };
     const auto tile = [](Kind k) { return k == kWide ? kWideRows : (k == kNarrow2 ? 32 : 16); };
-    const int64_t block = half ? kBlock<__bf16> : kBlock<float>, round = kWaves * block, wide_round = EV("X_WR", 4) * kWideKeys;
+    const int64_t block = half ? kBlock<__bf16> : kBlock<float>, round = kWaves * block, wide_round = 4 * kWideKeys;
 
     p.own = kind(own_rows);
     a.whole = a.B > 0 && p.own == kWide && rows >= kWideRows * a.B && a.prefix_len + room < INT32_MAX - 4096;
@@ -95,11 +103,16 @@ Plan plan(int num_cu, bool half,  int64_t max_added, int64_t max_length, int64_t
                            &a.o_splits, &a.o_chunk);
         }
         p.prefix_blocks = (int64_t)a.Hkv * a.p_tiles * a.p_splits;
+        // a wave for a request's own keys where there are few of them and many requests
+        if (a.B > 0 && p.own != kWide && max_length <= kSoloBlocks * block && own_items >= 4 * num_cu) {
+            a.solo = 1;
+            split_keys(1, block, max_length, &a.o_splits, &a.o_chunk);
+        }
     }
     if (a.B > 0) {
         const int64_t each = (int64_t)a.Hkv * (a.B + (a.whole ? 2 : 0)) * (a.o_splits > 0 ? a.o_splits : 1);
         while (a.o_tiles > 1 && each * a.o_tiles >= (1 << 22)) a.o_tiles = (a.o_tiles + 1) / 2;  // workgroups take several
-        p.own_blocks = a.o_splits > 0 ? each * a.o_tiles : 0;
+        p.own_blocks = a.o_splits > 0 ? ceil_div(each * a.o_tiles, a.solo ? kWaves : 1) : 0;
     }
     return p;
 }
@@ -214,7 +227,7 @@ void attention_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* q, pfr_dtype dtyp
     a.by_requests = by(a.B + (a.whole ? 2 : 0));
     // the workgroups that come last join the rows, where few enough requests share the prefix's
     if (a.part_o != nullptr && p.own != pfr::attn::kWide && p.own_blocks > 0 &&
-        (in_shares || !one || (B + 2 <= 64 && T * a.G <= 64)))
+        (in_shares || !one || (!a.solo && B + 2 <= 64 && T * a.G <= kJoinRows)))
         a.arrived = arrived;
     a.p_items = (int32_t)p.prefix_blocks;
     enqueue(ctx, kv, dtype, a, p.prefix, p.prefix_blocks + (one ? p.own_blocks : 0));

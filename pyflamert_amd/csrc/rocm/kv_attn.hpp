@@ -52,12 +52,13 @@ struct Args {
     int32_t B;
     // Apart: p_items = Hkv * p_tiles * p_splits workgroups for the prefix, p_chunk
     // keys a split, its tiles over the rows of all tokens; then Hkv * B *
-    // o_tiles * o_splits for the requests' own keys, o_chunk a split.
+    // o_tiles * o_splits for the requests' own keys, o_chunk a split, with a
+    // workgroup or (solo) a wave for each.
     // Together (whole, and in shares): a request's tiles see the prefix and then
     // its own keys.
     FastDiv by_heads, by_p_tiles, by_o_tiles, by_requests, by_fours;  // by_fours: by D / 4
     int32_t shares, parts, items;  // of a key head: workgroups, parts of a tile of rows at most, tiles at most
-    int32_t whole, p_items, p_tiles, p_splits, p_chunk, o_tiles, o_splits, o_chunk;
+    int32_t whole, solo, p_items, p_tiles, p_splits, p_chunk, o_tiles, o_splits, o_chunk;
     const char* zeros;  // 256 of them
     float* part_o;    // [p_splits + o_splits][T * Hq][D], null: rows are whole after one workgroup
     float2* part_ml;  // [p_splits + o_splits][T * Hq]: the score weighed against (log2 units), sum of weights
@@ -66,7 +67,7 @@ struct Args {
     uint32_t* arrived;  // [Hkv][B + 2]; in shares [Hkv][items], by tile of rows
 };
 
-// The kernels: narrow (kNarrow1, 2: 16 or 32 rows, waves share the keys) and
+// The kernels: narrow (kNarrow1, 2: 16 or, of 16-bit types, 32 rows, waves share the keys) and
 // wide (kWideRows rows, waves share a tile of keys), and wide in equal shares.
 enum Kind { kNarrow1, kNarrow2, kWide, kShares };
 
@@ -385,11 +386,11 @@ __device__ __forceinline__ s4 read_tr(unsigned lds) {
 // One workgroup's rows against keys [lo, hi) of one table.  Rows r0 .. of the
 // n_rows that start at token t0: row r is query head r % G of token t0 + r / G.
 // lim0 and per_token: row r sees keys below lim0 + per_token * (r / G).
-// Writes the rows' part `part`.  found: id0 is the table's entry for the lane's key of
+// Writes the rows' part `part`.  solo: a wave's work, not a workgroup's.  found: id0 is the table's entry for the lane's key of
 // the wave's first block already.
 template <class QT, class KT, int DP, int RT, bool FULL>
 __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0, int r0, int n_rows,
-                                       const Seg& seg, int lim0, int per_token, int part, bool found, int32_t id0) {
+                                       const Seg& seg, int lim0, int per_token, int part, bool solo, bool found, int32_t id0) {
     const int32_t* __restrict__ table = seg.table;
     const int lo = seg.lo, hi = seg.hi;
     typedef Tiles<QT, KT, DP, RT, FULL> TT;
@@ -421,8 +422,7 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
     // lane i (modulo a block) finds key i of a block: its table entry, and once that is there its offset
     constexpr int kB = kBlock<QT>, NJ = TT::NJ;
     constexpr uint32_t kAll = ~0u >> (32 - kB);
-    constexpr int step = kWaves * kB;
-    const int first = lo + w * kB;
+    const int step = solo ? kB : kWaves * kB, first = solo ? lo : lo + w * kB;
     const auto find = [&](int k0) { return key_place(a.map, k0 + (lane & (kB - 1)), hi); };
     const auto offset = [&](int k0, const KeyPlace& at, int32_t id) { return key_offset(a.map, at, id, k0 + (lane & (kB - 1)), hi); };
     const auto load_k = [&](int64_t off) {
@@ -536,6 +536,28 @@ __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0,
     n = here(n);
     g = here(g);
     const int64_t rows_all = (int64_t)a.T * a.Hq;
+    if (solo) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int r = r0 + rt * 16 + n, dt = (int)a.group.div((uint32_t)r);
+            l[rt] = row_sum(l[rt]);
+            if (r >= n_rows) continue;
+            const int64_t at = (int64_t)part * rows_all + (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G);
+            if (g == 0) put_pair(a.part_ml + at, m[rt], l[rt]);
+#pragma unroll
+            for (int c = 0; c < TT::CC; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < TT::VV; e += 4) {
+                        const int d = (16 * c + 4 * g + i) * TT::VV + e;
+                        if (FULL || d < a.D)
+                            put_four(a.part_o + at * a.D + d, f4{x.o[rt][c * TT::VV + e][i], x.o[rt][c * TT::VV + e + 1][i],
+                                                                 x.o[rt][c * TT::VV + e + 2][i], x.o[rt][c * TT::VV + e + 3][i]});
+                    }
+        }
+        return;
+    }
     // the waves' sums, joined
     float* sm = lds;                       // [kWaves][16 RT] maxima
     float* sl = lds + kWaves * 16 * RT;    // [kWaves][16 RT] sums
@@ -1035,6 +1057,7 @@ __device__ __forceinline__ Item item_of(const Args& a) {
         return x;
     }
     i -= a.p_items;
+    if (a.solo) i = i * kWaves + (uint32_t)uniform((int)threadIdx.x >> 6);
     x.h = next(a.by_heads);
     x.tile = next(a.by_o_tiles);
     x.b = next(a.by_requests);
@@ -1044,19 +1067,20 @@ __device__ __forceinline__ Item item_of(const Args& a) {
 
 // No keys for rows [r0, r1) of a part: the join skips what has no weight.
 __device__ __forceinline__ void no_keys(const Args& a, int h, int t0, int r0, int r1, int part) {
-    for (int r = r0 + (int)threadIdx.x; r < r1; r += (int)blockDim.x) {
+    const int lanes = a.solo && part >= a.p_splits ? 64 : (int)blockDim.x;
+    for (int r = r0 + ((int)threadIdx.x & (lanes - 1)); r < r1; r += lanes) {
         const int dt = (int)a.group.div((uint32_t)r);
         put_pair(a.part_ml + (int64_t)part * a.T * a.Hq + (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G), -INFINITY, 0.0f);
     }
 }
 
-// A workgroup joins the rows of request b, or of the tokens of none (b = B, B + 1).
+// Waves `w`, w + n, .. of the rows of request b, or of the tokens of none (b = B, B + 1), are joined.
 template <class QT>
-__device__ __forceinline__ void join_rows(const Args& a, int h, int b) {
+__device__ __forceinline__ void join_rows(const Args& a, int h, int b, int w, int n) {
     int t0, t1;
     tokens_of(a.start, a.B, b, a.T, &t0, &t1);
     const int parts = a.p_splits + (b < a.B ? a.o_splits : 0);
-    for (int r = (int)threadIdx.x >> 6; r < (t1 - t0) * a.G; r += kWaves) {
+    for (int r = w; r < (t1 - t0) * a.G; r += n) {
         const int dt = (int)a.group.div((uint32_t)r);
         join_row<QT, true>(a, (int64_t)(t0 + dt) * a.Hq + h * a.G + (r - dt * a.G), t0 + dt, parts);
     }
@@ -1088,7 +1112,27 @@ __device__ __forceinline__ void arrive(const Args& a, int h, int b, unsigned lon
         if (lane == 0) *flags = mask;
     }
     __syncthreads();
-    for (unsigned long long mask = uniform(*flags); mask; mask &= mask - 1) join_rows<QT>(a, h, b < 0 ? __builtin_ctzll(mask) : b);
+    // one row a request: a wave each; else the waves share a request's
+    int i = 0;
+    for (unsigned long long mask = uniform(*flags); mask; mask &= mask - 1, ++i) {
+        const int r = b < 0 ? __builtin_ctzll(mask) : b;
+        join_rows<QT>(a, h, r, (w + i) % kWaves, kWaves);
+    }
+}
+
+// The same for a wave that wrote its part alone, after an earlier launch's for the prefix.
+template <class QT>
+__device__ __forceinline__ void arrive_alone(const Args& a, int h, int b) {
+    __builtin_amdgcn_s_waitcnt(0);
+    bool last = true;
+    if (a.o_tiles * a.o_splits > 1) {
+        int old = 0;
+        uint32_t* at = a.arrived + (int64_t)h * (a.B + 2) + b;
+        if ((threadIdx.x & 63) == 0) old = (int)__hip_atomic_fetch_add(at, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = uniform(old) + 1 == a.o_tiles * a.o_splits;
+        if (last && (threadIdx.x & 63) == 0) __hip_atomic_store(at, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (last) join_rows<QT>(a, h, b, 0, 1);
 }
 
 // The narrow form (DN columns, FULL: all of them there, RT tiles of rows) or, with
@@ -1096,7 +1140,8 @@ __device__ __forceinline__ void arrive(const Args& a, int h, int b, unsigned lon
 template <class QT, class KT, int DN, bool FULL, int RT, int DW, bool WF>
 __device__ __forceinline__ void attention(const Args& a, char* lds) {
     const Item x = item_of(a);
-    const bool prefix = x.b < 0;
+    if (x.b >= 0 && x.split >= a.o_splits) return;  // a wave of its own past the last item
+    const bool prefix = x.b < 0, solo = DW == 0 && a.solo && !prefix;
     int t0 = 0, t1 = a.T, lim0 = a.prefix_len, P = a.prefix_len, part = x.split, tiles_apart = a.p_tiles;
     int64_t room = 0;
     const int32_t* table = nullptr;
@@ -1112,7 +1157,7 @@ __device__ __forceinline__ void attention(const Args& a, char* lds) {
             // the first keys' entries, while the request's length is on its way
             constexpr int kB = kBlock<QT>;
             first = x.split * a.o_chunk;
-            const int w = (int)threadIdx.x >> 6, key = first + w * kB + ((int)threadIdx.x & (kB - 1));
+            const int w = solo ? 0 : (int)threadIdx.x >> 6, key = first + w * kB + ((int)threadIdx.x & (kB - 1));
             id0 = table[key_place(a.map, key, (int)room).entry];
         }
         if (a.whole) tokens_of(a.start, a.B, x.b, a.T, &t0, &t1);
@@ -1145,16 +1190,19 @@ __device__ __forceinline__ void attention(const Args& a, char* lds) {
             wide<QT, DW, WF, false>(a, *reinterpret_cast<WideLds<DW>*>(lds), x.h, t0, r0, n_rows, pre, own, lim0, part);
         } else {
             narrow<QT, KT, DN, RT, FULL>(a, reinterpret_cast<float*>(lds), x.h, t0, r0, n_rows, prefix ? pre : own, lim0, prefix ? 0 : 1, part,
-                                         lo == first, id0);
-            __syncthreads();
+                                         solo, lo == first, id0);
+            if (!solo) __syncthreads();
         }
     }
     if constexpr (DW == 0) {
         if (a.arrived != nullptr) {
-            if (n_rows > 0) arrive<QT>(a, x.h, x.b, reinterpret_cast<unsigned long long*>(lds));
+            if (n_rows > 0) {
+                if (solo) arrive_alone<QT>(a, x.h, x.b);
+                else arrive<QT>(a, x.h, x.b, reinterpret_cast<unsigned long long*>(lds));
+            }
             // nothing else of this launch comes to the tokens of no request
             if (a.p_items == 0 && x.b == 0 && x.tile == 0 && x.split == 0)
-                for (int b = a.B; b < a.B + 2; ++b) join_rows<QT>(a, x.h, b);
+                for (int b = a.B; b < a.B + 2; ++b) join_rows<QT>(a, x.h, b, solo ? 0 : (int)threadIdx.x >> 6, solo ? 1 : kWaves);
         }
     }
 }
@@ -1382,7 +1430,7 @@ void launch_kind(hipStream_t s, const Args& a, Kind kind, unsigned blocks) {
         if (kind == kShares) { hipLaunchKernelGGL((k_attn_shares<QT, DW, WF>), grid, dim3(kWideWaves * 64), 0, s, a); return; }
         if (kind == kWide) { hipLaunchKernelGGL((k_attn_wide<QT, DW, WF>), grid, dim3(kWideWaves * 64), 0, s, a); return; }
     }
-    if constexpr (DN < 256) {
+    if constexpr (DN < 256 && sizeof(QT) == 2) {
         if (kind == kNarrow2) { hipLaunchKernelGGL((k_attn_narrow<QT, KT, DN, FULL, 2>), grid, wg, 0, s, a); return; }
     }
     hipLaunchKernelGGL((k_attn_narrow<QT, KT, DN, FULL, 1>), grid, wg, 0, s, a);

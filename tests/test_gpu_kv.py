@@ -506,6 +506,22 @@ def test_step_on_another_stream_and_in_a_graph(ctx):
         ctx.set_stream(old)
 
 
+@pytest.mark.parametrize("q,cache", TYPES)
+@pytest.mark.parametrize("name", ["steps", "steps behind a prefix", "pieces of prompts"])
+def test_attention_of_many_short_requests(ctx, q, cache, name):
+    """More requests than the chip takes workgroups, each of a few keys; passes
+    give the same bits."""
+    heads, kvh, dim, prefix, lengths, added = {
+        "steps": (8, 8, 128, 0, [1 + i % 30 for i in range(150)], [1] * 150),
+        "steps behind a prefix": (8, 8, 64, 70, [1 + i % 20 for i in range(140)], [1] * 140),
+        "pieces of prompts": (8, 8, 80, 0, [i % 21 + i % 9 for i in range(70)], [i % 21 for i in range(70)]),
+    }[name]
+    c = Case(heads, kvh, dim, 8, "head", q, cache, prefix, lengths, added)
+    first = c.check(ctx)
+    for _ in range(5):
+        assert torch.equal(bits(first), bits(c.run(ctx)))
+
+
 def test_attention_repeats_bit_for_bit(ctx):
     c = Case(16, 2, 128, 16, "head", "f16", "f16", 2000, [300, 900, 40, 700] * 4, [1] * 16)
     first = c.run(ctx)
