@@ -39,6 +39,10 @@ void clear_last_error();
 inline void require(bool ok, const std::string& msg) {
     if (!ok) throw Error(PFR_ERR_INVALID_ARG, msg);
 }
+// A literal becomes a string only where it is thrown.
+inline void require(bool ok, const char* msg) {
+    if (!ok) throw Error(PFR_ERR_INVALID_ARG, msg);
+}
 
 // Runs f and converts exceptions into a C status + thread-local message.
 template <class F>
