@@ -97,7 +97,10 @@ __device__ __forceinline__ int last_at_most(const int64_t* s, int64_t v) {
 // Grid (groups of kTabThreads requests) x (slices of a group's tokens and new
 // pages).  Every workgroup sums what the requests before its group take, scans
 // its own group's, and fills its slice; nothing passes between workgroups, so
-// one launch does it.
+// one launch does it.  A dependent chain of loads is what it costs (counts, then
+// pages, each about 1 us away), not bytes: 64 requests of one token 5.3 us,
+// 2048 prompts of 0 to 512 tokens 9.0 us for 4.5 MB; a call from the host takes
+// 7 us in either case.
 __global__ __launch_bounds__(kTabThreads) void k_kv_tables(TablesArgs a) {
     __shared__ int64_t tok[kTabThreads + 1], pg[kTabThreads + 1];
     __shared__ int32_t s_cached[kTabThreads], s_have[kTabThreads];
@@ -244,7 +247,10 @@ __device__ __forceinline__ void copy8(const S* __restrict__ src, C* __restrict__
     *reinterpret_cast<CV*>(dst) = __builtin_convertvector(s, CV);
 }
 
-// One 8-element vector of the keys and of the values per thread.
+// One 8-element vector of the keys and of the values per thread: all loads are in
+// flight at once, and a page's rows are written in whole 16-byte vectors.  Bound
+// by memory: 16384 tokens of 32 heads of 128, bf16, 91 us for 537 MB, 5.9 TB/s
+// where a large copy reaches 4.8; small steps are a launch (3 us, 7 for the host).
 template <class S, class C>
 __global__ __launch_bounds__(256) void k_kv_write(WriteArgs a) {
     const int64_t base = (int64_t)blockIdx.x * 256;

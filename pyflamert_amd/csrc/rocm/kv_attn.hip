@@ -91,15 +91,21 @@ Plan plan(int num_cu, bool half, int64_t max_added, int64_t max_length, int64_t 
         a.o_tiles = a.B > 0 ? (int32_t)ceil_div(own_rows, tile(p.own)) : 0;
         const int64_t prefix_items = (int64_t)a.Hkv * a.p_tiles, own_items = (int64_t)a.Hkv * a.B * a.o_tiles;
         if (p.prefix != kWide && p.own != kWide) {
-            // chunks of one size, four workgroups to a CU if all requests were of max_length
+            // Chunks of one size, four workgroups to a CU if all requests were of
+            // max_length; two with float32 rows, whose few keys a round and
+            // longer start want more keys to a workgroup (8 requests, 32
+            // heads of 128 behind 4096 keys, float32: 64 us with four, 58 so).
             const int64_t keys = prefix_items * a.prefix_len + own_items * max_length;
-            const int64_t c = ceil_div(ceil_div(keys, 4 * num_cu), round) * round;
+            const int64_t c = ceil_div(ceil_div(keys, (half ? 4 : 2) * num_cu), round) * round;
             split_keys(ceil_div(a.prefix_len, c), round, a.prefix_len, &a.p_splits, &a.p_chunk);
             split_keys(ceil_div(max_length, c), round, max_length, &a.o_splits, &a.o_chunk);
         } else {
             split_keys(ceil_div(num_cu, prefix_items), wide_round, a.prefix_len, &a.p_splits, &a.p_chunk);
+            // one wide workgroup fills a CU; narrow ones eight to a CU, so that
+            // requests of uneven lengths even out (128 requests of up to 2048
+            // keys, 8 heads: 224 us with four, 220 so)
             if (a.B > 0)
-                split_keys(ceil_div((p.own == kWide ? 1 : 4) * num_cu, own_items), p.own == kWide ? wide_round : round, max_length,
+                split_keys(ceil_div((p.own == kWide ? 1 : 8) * num_cu, own_items), p.own == kWide ? wide_round : round, max_length,
                            &a.o_splits, &a.o_chunk);
         }
         p.prefix_blocks = (int64_t)a.Hkv * a.p_tiles * a.p_splits;

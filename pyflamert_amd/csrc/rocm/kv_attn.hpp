@@ -386,8 +386,17 @@ __device__ __forceinline__ s4 read_tr(unsigned lds) {
 // One workgroup's rows against keys [lo, hi) of one table.  Rows r0 .. of the
 // n_rows that start at token t0: row r is query head r % G of token t0 + r / G.
 // lim0 and per_token: row r sees keys below lim0 + per_token * (r / G).
-// Writes the rows' part `part`.  solo: a wave's work, not a workgroup's.  found: id0 is the table's entry for the lane's key of
-// the wave's first block already.
+// Writes the rows' part `part`.  solo: a wave's work, not a workgroup's.  found:
+// id0 is the table's entry for the lane's key of the wave's first block already.
+//
+// The form of single tokens, whose own keys nobody else reads: bound by memory.
+// A wave takes every fourth block of keys straight into registers, for nothing
+// of a block is used twice, and the four waves' sums meet once, at the end.
+// 64 requests of 32 heads of 128, 512 keys each on average, bf16: 110 us, 4.9
+// TB/s where a large copy reaches 4.8 and reading alone 6.2.  Float32 rows
+// take the float32 products (154 TFLOP/s) on keys and values widened in
+// registers: 4.6 TB/s on a float32 cache, 2.4 on a bf16 one, whose
+// keys come twice as fast (blocks of 32 keys there: 34 us against 29).
 template <class QT, class KT, int DP, int RT, bool FULL>
 __device__ __forceinline__ void narrow(const Args& a, float* lds, int h, int t0, int r0, int n_rows,
                                        const Seg& seg, int lim0, int per_token, int part, bool solo, bool found, int32_t id0) {
@@ -664,6 +673,14 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // and O^T = V^T P^T in 32x32x16 products, so that a row's scores, its weights
 // and its column of O^T stay in the lanes n and n + 32.  The second product of
 // a tile runs beside the exponentials of the next.
+//
+// Bound by instruction issue: a tile's 64 x 32 scores of a wave cost about as many
+// cycles of vector work (exponentials, running maximum, rounding) as of matrix
+// work, and two waves to a SIMD overlap most of it: 128 tokens of 8 query heads a
+// key head against 16384 keys, f16, 91 us, 755 TFLOP/s, where a large product
+// reaches 1100; matrix unit busy 40 % of the cycles, no LDS bank conflicts.  With
+// few rows it is bound by memory: 64 rows against 8192 keys of 32 heads, 31 us,
+// 4.3 TB/s.  Staggered waves and raised wave priorities gave nothing.
 template <class T, int DP, bool FULL, bool SHARED>
 __device__ __forceinline__ void wide(const Args& a, WideLds<DP>& lds, int h, int t0, int r0, int n_rows, const Seg& pre,
                                      const Seg& own, int lim0, int part) {
@@ -1303,6 +1320,8 @@ __device__ __forceinline__ void join_tile(const Args& a, float* weight, int h, i
 // keys, laid end to end in units of 64 keys and cut into equal shares, one a
 // workgroup: with a tile to a workgroup, 2.2 tiles to a CU took as long as
 // three.  A tile that is cut is joined by the workgroup that comes last to it.
+// 16 prompts of up to 512 tokens behind 4096 keys, 32 heads on 8, bf16: 406 us
+// with a tile to a workgroup, 354 so, 811 TFLOP/s.
 template <class T, int DW, bool WF>
 __device__ __forceinline__ void shares(const Args& a, WideLds<DW>& lds, ShareLds& sh) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, nb = a.B + 2;
