@@ -454,9 +454,12 @@ int pfr_kv_write_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* k, const void* 
  * max_added and max_length bound the tokens and the length of a request as the
  * caller knows them (0: as many as T and the table allow); they shape the
  * launch only, and results are right without them.
- * Partial sums go through the context's grow-only scratch: capture only after
- * a call of the largest shape.  Device pointers; results do not depend on
- * timing. */
+ * One to three launches on the context's stream, nothing on the host.  Partial
+ * sums, and counters by which the last workgroup at a row knows to join them,
+ * lie in the context's grow-only scratch: capture only after a call of the
+ * largest shape, and let a change of the context's stream wait for the calls
+ * before it.  Device pointers; the parts are joined in one order whoever joins
+ * them, so the same call gives the same bits. */
 int pfr_kv_attention_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* q, pfr_dtype dtype, int64_t T,
                          int64_t heads, int64_t ldq, float scale, const int32_t* prefix_table,
                          int64_t prefix_len, const int32_t* table, int64_t table_w,

@@ -2,7 +2,8 @@
 MatMul/Gemm path.
 
 * ``pyflamert_amd.rocm`` -- numpy/pointer front-end of the C ABI
-  (include/pfr_rocm.h): CSR SpMM/SpMV, the Gemm form, 2:4 int8/bf16 GEMM.
+  (include/pfr_rocm.h): CSR SpMM/SpMV, the Gemm form, 2:4 int8/bf16 GEMM, and a paged key/value
+  cache (block tables, writes, attention behind a shared prefix).
 * the C++ runtime (InferenceSession / OperatorRegistry / RocmExecutor) lives
   in csrc/runtime and is reached through ``pyflamert_amd.session``.
 
