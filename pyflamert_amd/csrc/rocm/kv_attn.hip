@@ -46,6 +46,10 @@ constexpr int kSoloBlocks = 8;
 // take a launch, for that joins them side by side (14 rows of 24 parts: 87 us
 // in the workgroups, 24 so; 4 rows of 5: 9 us, 12 so).
 constexpr int kJoinRows = 8;
+// And parts of a row that they join behind a launch of its own for the prefix
+// (128 requests, 64 heads, 10 parts: 219 us, with a launch 214; 59 requests of
+// one head, 24 parts: 44 us, 31; 118 requests, 12 heads, 2 parts: 23 us, 25).
+constexpr int kJoinParts = 4;
 
 // The kernels of a call and their workgroups; one launch where both parts take the same kernel.
 struct Plan {
@@ -231,9 +235,9 @@ void attention_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* q, pfr_dtype dtyp
     a.by_o_tiles = by(a.o_tiles);
     a.by_fours = by(a.D / 4);
     a.by_requests = by(a.B + (a.whole ? 2 : 0));
-    // the workgroups that come last join the rows, where few enough requests share the prefix's
+    // the workgroups that come last join the rows, where there is little to join
     if (a.part_o != nullptr && p.own != pfr::attn::kWide && p.own_blocks > 0 &&
-        (in_shares || !one || (!a.solo && B + 2 <= 64 && T * a.G <= kJoinRows)))
+        (in_shares || (!one && parts <= kJoinParts) || (one && !a.solo && B + 2 <= 64 && T * a.G <= kJoinRows)))
         a.arrived = arrived;
     a.p_items = (int32_t)p.prefix_blocks;
     enqueue(ctx, kv, dtype, a, p.prefix, p.prefix_blocks + (one ? p.own_blocks : 0));
