@@ -522,6 +522,18 @@ def test_attention_of_many_short_requests(ctx, q, cache, name):
         assert torch.equal(bits(first), bits(c.run(ctx)))
 
 
+@pytest.mark.parametrize("q,cache", TYPES[:2])
+def test_attention_of_prompts_repeats_bit_for_bit(ctx, q, cache):
+    """Prompts whose tiles are cut between workgroups give the same bits from call to
+    call, other calls in between."""
+    c = Case(8, 1, 128, 16, "head", q, cache, 700, [290, 600, 31], [260, 333, 31])
+    other = Case(4, 2, 64, 16, "head", q, cache, 90, [50, 9], [1, 1])
+    first, first_other = c.check(ctx), other.check(ctx)
+    for _ in range(10):
+        assert torch.equal(bits(first), bits(c.run(ctx)))
+        assert torch.equal(bits(first_other), bits(other.run(ctx)))
+
+
 def test_attention_repeats_bit_for_bit(ctx):
     c = Case(16, 2, 128, 16, "head", "f16", "f16", 2000, [300, 900, 40, 700] * 4, [1] * 16)
     first = c.run(ctx)
