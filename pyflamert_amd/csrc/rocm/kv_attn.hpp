@@ -392,7 +392,7 @@ __device__ __forceinline__ s4 read_tr(unsigned lds) {
 // The form of single tokens, whose own keys nobody else reads: bound by memory.
 // A wave takes every fourth block of keys straight into registers, for nothing
 // of a block is used twice, and the four waves' sums meet once, at the end.
-// 64 requests of 32 heads of 128, 512 keys each on average, bf16: 110 us, 4.9
+// 64 requests of 32 heads of 128, 512 keys each on average, bf16: 107 us, 5.0
 // TB/s where a large copy reaches 4.8 and reading alone 6.2.  Float32 rows
 // take the float32 products (154 TFLOP/s) on keys and values widened in
 // registers: 4.6 TB/s on a float32 cache, 2.4 on a bf16 one, whose
@@ -677,7 +677,7 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // Bound by instruction issue: a tile's 64 x 32 scores of a wave cost about as many
 // cycles of vector work (exponentials, running maximum, rounding) as of matrix
 // work, and two waves to a SIMD overlap most of it: 128 tokens of 8 query heads a
-// key head against 16384 keys, f16, 91 us, 755 TFLOP/s, where a large product
+// key head against 16384 keys, f16, 88 us, 780 TFLOP/s, where a large product
 // reaches 1100; matrix unit busy 40 % of the cycles, no LDS bank conflicts.  With
 // few rows it is bound by memory: 64 rows against 8192 keys of 32 heads, 31 us,
 // 4.3 TB/s.  Staggered waves and raised wave priorities gave nothing.
