@@ -177,7 +177,7 @@ int main() {
         m.pages = 1 + r() % 9;
         m.token_stride = 8 * (1 + r() % 4);
         m.page_stride = m.token_stride * page + 8 * (r() % 3);
-        int32_t* t = (int32_t*)malloc(4 * (w ? w : 1));  // of its size, so that a checker sees a read past it
+        int32_t* t = (int32_t*)malloc(4 * (w ? w : 1));  // of its size, so that a read past it shows under a sanitizer
         for (int i = 0; i < w; ++i) t[i] = (int32_t)(r() % 4 ? r() % 12 : r()) - (r() % 5 == 0 ? 20 : 0);
         const int hi = w ? 1 + r() % (w * page) : 0;
         for (int key = 0; hi && key < (w + 2) * page; ++key) {
