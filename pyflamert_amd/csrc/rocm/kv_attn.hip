@@ -42,6 +42,13 @@ void split_keys(int64_t want, int64_t round, int64_t keys, int32_t* splits, int3
 // Own keys of so many blocks at most go to a wave each: with one to a workgroup,
 // 67 requests of one key, 32 heads, took 77 us, 36 so.
 constexpr int kSoloBlocks = 8;
+// And, of a 16-bit cache, up to so many keys where a CU's share is kSoloItems of one
+// tile of rows each: the waves then stand in for each other, and none waits for
+// the rest of its workgroup (200 requests, 32 heads, bf16, up to 301 keys: 151 us
+// with a workgroup to each, 107 so; up to 501: 186, 169; up to 701: 223, 228;
+// up to 1001: 291, 314.  300 requests of up to 301 keys in float32: 148, 154.
+// With half as many items, 64 requests of up to 1024 keys: 144, 164).
+constexpr int kSoloKeys = 512, kSoloItems = 16;
 // Rows of a key head that the workgroups that come last join themselves; more
 // take a launch, for that joins them side by side (14 rows of 24 parts: 87 us
 // in the workgroups, 24 so; 4 rows of 5: 9 us, 12 so).
@@ -58,7 +65,7 @@ struct Plan {
 };
 
 // Which kernels, and how the work is cut into workgroups.
-Plan plan(int num_cu, bool half, int64_t max_added, int64_t max_length, int64_t room, Args& a) {
+Plan plan(int num_cu, bool half, bool half_cache, int64_t max_added, int64_t max_length, int64_t room, Args& a) {
     using namespace pfr::attn;
     Plan p;
     const int64_t rows = (int64_t)a.T * a.G, own_rows = max_added * a.G;  // of a key head
@@ -113,8 +120,10 @@ Plan plan(int num_cu, bool half, int64_t max_added, int64_t max_length, int64_t 
                            &a.o_splits, &a.o_chunk);
         }
         p.prefix_blocks = (int64_t)a.Hkv * a.p_tiles * a.p_splits;
-        // a wave for a request's own keys where there are few of them and many requests
-        if (a.B > 0 && p.own != kWide && max_length <= kSoloBlocks * block && own_items >= 4 * num_cu) {
+        // a wave for a request's own keys where there are few of them and many requests, or very many of them
+        const bool few = max_length <= kSoloBlocks * block && own_items >= 4 * num_cu;
+        const bool many = half_cache && max_length <= kSoloKeys && a.o_tiles == 1 && own_items >= kSoloItems * num_cu;
+        if (a.B > 0 && p.own != kWide && (few || many)) {
             a.solo = 1;
             split_keys(1, block, max_length, &a.o_splits, &a.o_chunk);
         }
@@ -216,7 +225,7 @@ void attention_dev(pfr_ctx* ctx, const pfr_kv* kv, const void* q, pfr_dtype dtyp
     // bounds: what a request may add and hold
     if (max_added == 0 || max_added > T) max_added = T;
     if (max_length == 0 || max_length > room) max_length = room;
-    const Plan p = plan(ctx->num_cu, dtype != PFR_F32, max_added, max_length, room, a);
+    const Plan p = plan(ctx->num_cu, dtype != PFR_F32, kv->dtype != PFR_F32, max_added, max_length, room, a);
 
     const bool in_shares = p.own == pfr::attn::kShares;
     const int64_t parts = in_shares ? a.parts : a.p_splits + a.o_splits, rows = T * heads;

@@ -507,13 +507,14 @@ def test_step_on_another_stream_and_in_a_graph(ctx):
 
 
 @pytest.mark.parametrize("q,cache", TYPES)
-@pytest.mark.parametrize("name", ["steps", "steps behind a prefix", "pieces of prompts"])
+@pytest.mark.parametrize("name", ["steps", "steps behind a prefix", "steps of longer requests", "pieces of prompts"])
 def test_attention_of_many_short_requests(ctx, q, cache, name):
-    """More requests than the chip takes workgroups, each of a few keys; passes
+    """More requests than the chip takes workgroups, most of a few keys each; passes
     give the same bits."""
     heads, kvh, dim, prefix, lengths, added = {
         "steps": (8, 8, 128, 0, [1 + i % 30 for i in range(150)], [1] * 150),
         "steps behind a prefix": (8, 8, 64, 70, [1 + i % 20 for i in range(140)], [1] * 140),
+        "steps of longer requests": (32, 32, 64, 0, [1 + i * 37 % 500 for i in range(130)], [1] * 130),
         "pieces of prompts": (8, 8, 80, 0, [i % 21 + i % 9 for i in range(70)], [i % 21 for i in range(70)]),
     }[name]
     c = Case(heads, kvh, dim, 8, "head", q, cache, prefix, lengths, added)
