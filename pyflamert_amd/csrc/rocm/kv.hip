@@ -249,8 +249,8 @@ __device__ __forceinline__ void copy8(const S* __restrict__ src, C* __restrict__
 
 // One 8-element vector of the keys and of the values per thread: all loads are in
 // flight at once, and a page's rows are written in whole 16-byte vectors.  Bound
-// by memory: 16384 tokens of 32 heads of 128, bf16, 91 us for 537 MB, 5.9 TB/s
-// where a large copy reaches 4.8; small steps are a launch (3 us, 7 for the host).
+// by memory: 16384 tokens of 32 heads of 128, bf16, 91 to 98 us for 537 MB, 5.5 to
+// 5.9 TB/s where a large copy reaches 4.8; small steps are a launch (3 us, 7 for the host).
 template <class S, class C>
 __global__ __launch_bounds__(256) void k_kv_write(WriteArgs a) {
     const int64_t base = (int64_t)blockIdx.x * 256;
